@@ -445,6 +445,127 @@ typedef struct snn_train_io {
 } snn_train_io;
 int snn_train_step_grad(const snn_cfg *cfg, const snn_train_io *io, void *stream);
 
+/* ---- gradient clipping ------------------------------------------------------ */
+/*
+ * Global norm over many gradient tensors and clipping by it (torch.nn.utils.clip_grad_norm_ semantics; no counterpart in
+ * the reference).  src / numel / dtype (SNN_DT_*): HOST arrays of n_tensors entries; every tensor is a dense block of numel
+ * elements, in any alignment.
+ *   norm = grad_scale (sum |g|^p)^(1/p), norm_type 1, 2, or 0 for the largest magnitude;  coef = min(1, max_norm / (norm + 1e-6))
+ *   out[0] = norm, out[1] = coef (device floats);  dst[i] = src[i] * coef if dst != NULL (dst[i] may be src[i])
+ * Sums are fp64 in an order that depends on the sizes alone.  Not finite gradients give the norm and the products IEEE
+ * arithmetic gives.  scratch: snn_clip_scratch_doubles(n_tensors, numel) doubles.
+ * grad_scale: what the optimizer will multiply gradients by (1 / world size after a data-parallel sum).
+ */
+int64_t snn_clip_scratch_doubles(int32_t n_tensors, const int64_t *numel);
+int snn_clip_grads(int32_t n_tensors, const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtype,
+                   int32_t norm_type, float max_norm, float grad_scale, float *out, double *scratch, int64_t scratch_doubles,
+                   void *stream);
+/* snn_adam_step / snn_sgd_step with the gradients multiplied by grad_scale * *coef, coef a device float (out + 1 above). */
+int snn_adam_step_clipped(int64_t n, float *params, const float *grads, float *exp_avg, float *exp_avg_sq, int64_t step,
+                          float lr, float beta1, float beta2, float eps, float weight_decay, float grad_scale,
+                          const float *coef, void *stream);
+int snn_sgd_step_clipped(int64_t n, float *params, const float *grads, float *momentum_buf, int64_t step, float lr,
+                         float momentum, float weight_decay, float grad_scale, const float *coef, void *stream);
+
+/* ---- sequence operators: short causal convolution, selective scan ---------- */
+/*
+ * A recurrence that is linear in its state, h_t = a_t h_{t-1} + b_t with decays computed from the input (selective scan),
+ * and the depthwise convolution over the last few steps that stands in front of it: the other recurrence, besides the LSTM
+ * stack above, a sequence classifier or generator is built from.  No counterpart in the reference.
+ *
+ * Element types of the sequence tensors (x, delta, z, B, C, y and their gradients, convolution states): one type per call;
+ * parameters, their gradients and scan states are fp32.
+ */
+#define SNN_DT_F32 0
+#define SNN_DT_BF16 1
+#define SNN_DT_F16 2
+
+/*
+ * A batch of sequences.  Padded (offsets == NULL): n_seq sequences of at most max_T steps, lengths (n_seq, DEVICE) or NULL
+ * (all max_T).  Ragged rows (offsets != NULL, lengths == NULL): n_rows concatenated rows, sequence b holds rows
+ * [offsets[b], offsets[b + 1]) (n_seq + 1 entries, DEVICE), none longer than max_T.  The device arrays are read by the
+ * kernels only; values out of range are cut to the tensors (a length to [0, max_T], an offset to [0, n_rows]).
+ * Rows that belong to no step -- behind a sequence's end in a padded batch, outside every sequence among ragged rows, past
+ * max_T -- are never read, and zero in every output.  A sequence of length 0 hands its initial state on.
+ */
+typedef struct snn_seq {
+    int32_t n_seq, max_T;
+    int64_t n_rows;
+    const int32_t *lengths;
+    const int64_t *offsets;
+} snn_seq;
+
+/* element (sequence n, step t, channel d) is p[t * stride_t + n * stride_n + d] (strides in elements; ragged rows: the row
+ * is offsets[n] + t and stride_n is 0) */
+typedef struct snn_view {
+    void *p;
+    int64_t stride_t, stride_n;
+} snn_view;
+
+/*
+ * Depthwise causal convolution of `width` (2..4) taps, y = act(bias + sum_w weight[d][w] x[t - width + 1 + w]), act = silu
+ * or none.  Steps before the first come from state_in (n_seq, width - 1, channels; NULL: zeros); state_out receives the
+ * last width - 1 inputs of every sequence (state_in included where the sequence is shorter) and must not alias state_in.
+ * snn_conv_backward: dy, and dstate_out (gradient of state_out) or NULL -> dx, dweight (channels, width), dbias (or NULL),
+ * dstate_in (or NULL).  Sums over sequences and steps are taken in a fixed order, the last stage in fp64.  ws:
+ * snn_conv_workspace_bytes(args) bytes, 8-byte aligned.
+ */
+typedef struct snn_conv_args {
+    snn_seq seq;
+    int32_t dtype, channels, width, silu;
+    snn_view x, y, dy, dx;
+    const float *weight, *bias;
+    const void *state_in;
+    void *state_out;
+    const void *dstate_out;
+    void *dstate_in;
+    float *dweight, *dbias;
+    void *ws;
+    int64_t ws_bytes;
+} snn_conv_args;
+int snn_conv_forward(const snn_conv_args *args, void *stream);
+int64_t snn_conv_workspace_bytes(const snn_conv_args *args);
+int snn_conv_backward(const snn_conv_args *args, void *stream);
+/* One step of n_seq sequences: x, y (n_seq, channels) with row stride stride_n; state_in -> state_out, which may be the
+ * same buffer. */
+int snn_conv_step(const snn_conv_args *args, void *stream);
+
+/*
+ * Selective scan over `channels` channels of `states` (1..64) states each, in `groups` groups of channels that share B, C:
+ *   s_t = softplus(delta_t + delta_bias) (softplus == 0: delta_t + delta_bias)
+ *   h_t = exp(s_t A) h_{t-1} + s_t x_t B_t        h (channels, states), fp32, from state_in (n_seq, channels, states) or 0
+ *   y_t = (sum_n C_t h_t + skip x_t) * (z ? silu(z_t) : 1)
+ * A (channels, states); skip, delta_bias (channels) or NULL.  B, C: element (n, t, g, k) at
+ * p[t * stride_t + n * stride_n + g * stride_g + k].  state_out (n_seq, channels, states) or NULL receives the last states.
+ * tape: NULL, or snn_scan_tape_floats floats (16-byte aligned) that receive what the backward pass starts from.
+ * ws: snn_scan_workspace_bytes(args, backward) bytes, 16-byte aligned (may be 0).
+ */
+typedef struct snn_scan_args {
+    snn_seq seq;
+    int32_t dtype, channels, states, groups, softplus, reserved;
+    snn_view x, delta, z, B, C, y;
+    int64_t B_stride_g, C_stride_g;
+    const float *A, *skip, *delta_bias, *state_in;
+    float *state_out, *tape;
+    int64_t tape_floats;
+    /* backward: dstate_out = gradient of state_out or NULL.  dB, dC are laid out (row, group, state) with row = the view's
+     * and stride_g = states.  dskip, ddelta_bias, dstate_in may be NULL. */
+    snn_view dy, dx, ddelta, dz, dB, dC;
+    const float *dstate_out;
+    float *dA, *dskip, *ddelta_bias, *dstate_in;
+    void *ws;
+    int64_t ws_bytes;
+} snn_scan_args;
+int64_t snn_scan_tape_floats(const snn_scan_args *args);
+int64_t snn_scan_workspace_bytes(const snn_scan_args *args, int32_t backward);
+int snn_scan_forward(const snn_scan_args *args, void *stream);
+/* Gradients of a scalar loss from dy = dloss/dy (and dstate_out) and the tape of snn_scan_forward over the same inputs.
+ * Deterministic: every sum is taken in an order that depends on the sizes alone. */
+int snn_scan_backward(const snn_scan_args *args, void *stream);
+/* One step of n_seq sequences: x, delta, z, y (n_seq, channels), B, C (n_seq, groups, states), row stride stride_n;
+ * state_in -> state_out, which may be the same buffer. */
+int snn_scan_step(const snn_scan_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

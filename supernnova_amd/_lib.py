@@ -14,6 +14,7 @@ SNN_POOL_MEAN, SNN_POOL_STANDARD = 0, 1
 SNN_PREC_F32, SNN_PREC_BF16X3, SNN_PREC_F16X2 = 0, 1, 2
 SNN_CELL_LSTM, SNN_CELL_GRU, SNN_CELL_RNN = 0, 1, 2
 SNN_MASK_NONE, SNN_MASK_ARRAYS, SNN_MASK_PHILOX = 0, 1, 2
+SNN_DT_F32, SNN_DT_BF16, SNN_DT_F16 = 0, 1, 2
 BBB_EPS, BBB_MFE, BBB_PHILOX = 0, 1, 2
 TILE = 32
 
@@ -58,6 +59,37 @@ class SnnTrainIO(ctypes.Structure):
                 ("dw", ctypes.c_void_p), ("grad", ctypes.c_void_p),
                 ("fwd_ws", ctypes.c_void_p), ("fwd_ws_bytes", ctypes.c_int64),
                 ("bwd_ws", ctypes.c_void_p), ("bwd_ws_bytes", ctypes.c_int64)]
+
+
+class SnnSeq(ctypes.Structure):
+    """snn_seq of include/snn_hip.h (as the next three)."""
+    _fields_ = [("n_seq", ctypes.c_int32), ("max_T", ctypes.c_int32), ("n_rows", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("offsets", ctypes.c_void_p)]
+
+
+class SnnView(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("stride_t", ctypes.c_int64), ("stride_n", ctypes.c_int64)]
+
+
+class SnnConvArgs(ctypes.Structure):
+    _fields_ = [("seq", SnnSeq), ("dtype", ctypes.c_int32), ("channels", ctypes.c_int32), ("width", ctypes.c_int32),
+                ("silu", ctypes.c_int32), ("x", SnnView), ("y", SnnView), ("dy", SnnView), ("dx", SnnView),
+                ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("state_in", ctypes.c_void_p),
+                ("state_out", ctypes.c_void_p), ("dstate_out", ctypes.c_void_p), ("dstate_in", ctypes.c_void_p),
+                ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p), ("ws", ctypes.c_void_p), ("ws_bytes", ctypes.c_int64)]
+
+
+class SnnScanArgs(ctypes.Structure):
+    _fields_ = [("seq", SnnSeq), ("dtype", ctypes.c_int32), ("channels", ctypes.c_int32), ("states", ctypes.c_int32),
+                ("groups", ctypes.c_int32), ("softplus", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("x", SnnView), ("delta", SnnView), ("z", SnnView), ("B", SnnView), ("C", SnnView), ("y", SnnView),
+                ("B_stride_g", ctypes.c_int64), ("C_stride_g", ctypes.c_int64),
+                ("A", ctypes.c_void_p), ("skip", ctypes.c_void_p), ("delta_bias", ctypes.c_void_p), ("state_in", ctypes.c_void_p),
+                ("state_out", ctypes.c_void_p), ("tape", ctypes.c_void_p), ("tape_floats", ctypes.c_int64),
+                ("dy", SnnView), ("dx", SnnView), ("ddelta", SnnView), ("dz", SnnView), ("dB", SnnView), ("dC", SnnView),
+                ("dstate_out", ctypes.c_void_p), ("dA", ctypes.c_void_p), ("dskip", ctypes.c_void_p),
+                ("ddelta_bias", ctypes.c_void_p), ("dstate_in", ctypes.c_void_p),
+                ("ws", ctypes.c_void_p), ("ws_bytes", ctypes.c_int64)]
 
 
 class SnnError(RuntimeError):
@@ -117,6 +149,20 @@ SIGNATURES = {
     "snn_adam_step": (ctypes.c_int, [ctypes.c_int64, _P, _P, _P, _P, ctypes.c_int64] + [ctypes.c_float] * 6 + [_P]),
     "snn_train_step_grad": (ctypes.c_int, [_CFG, ctypes.POINTER(SnnTrainIO), _P]),
     "snn_sgd_step": (ctypes.c_int, [ctypes.c_int64, _P, _P, _P, ctypes.c_int64] + [ctypes.c_float] * 4 + [_P]),
+    "snn_clip_scratch_doubles": (ctypes.c_int64, [ctypes.c_int32, _P]),
+    "snn_clip_grads": (ctypes.c_int, [ctypes.c_int32, _P, _P, _P, _P, ctypes.c_int32, ctypes.c_float, ctypes.c_float, _P, _P,
+                                      ctypes.c_int64, _P]),
+    "snn_adam_step_clipped": (ctypes.c_int, [ctypes.c_int64, _P, _P, _P, _P, ctypes.c_int64] + [ctypes.c_float] * 6 + [_P, _P]),
+    "snn_sgd_step_clipped": (ctypes.c_int, [ctypes.c_int64, _P, _P, _P, ctypes.c_int64] + [ctypes.c_float] * 4 + [_P, _P]),
+    "snn_conv_forward": (ctypes.c_int, [ctypes.POINTER(SnnConvArgs), _P]),
+    "snn_conv_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(SnnConvArgs)]),
+    "snn_conv_backward": (ctypes.c_int, [ctypes.POINTER(SnnConvArgs), _P]),
+    "snn_conv_step": (ctypes.c_int, [ctypes.POINTER(SnnConvArgs), _P]),
+    "snn_scan_tape_floats": (ctypes.c_int64, [ctypes.POINTER(SnnScanArgs)]),
+    "snn_scan_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(SnnScanArgs), ctypes.c_int32]),
+    "snn_scan_forward": (ctypes.c_int, [ctypes.POINTER(SnnScanArgs), _P]),
+    "snn_scan_backward": (ctypes.c_int, [ctypes.POINTER(SnnScanArgs), _P]),
+    "snn_scan_step": (ctypes.c_int, [ctypes.POINTER(SnnScanArgs), _P]),
 }
 
 _lib = None

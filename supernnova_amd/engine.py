@@ -4,6 +4,7 @@ batching plan, and launches the kernels on torch's current HIP stream.
 PyTorch is plumbing here (allocator, streams); all arithmetic of the hot path
 runs in libsnn_hip.so.  Nothing in this module computes on the CPU.
 """
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -20,6 +21,11 @@ def _ptr(t):
 
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _on_device(device):
+    """Context in which launches go to `device`'s current stream (nothing to do where it is the current device)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _require_cuda(t, name):
@@ -510,20 +516,119 @@ def ce_loss_grad(logits, target, grad_scale=None):
     return buf[0], dlogits
 
 
+_DTYPES = {torch.float32: L.SNN_DT_F32, torch.bfloat16: L.SNN_DT_BF16, torch.float16: L.SNN_DT_F16}
+_NORM_TYPES = {1.0: 1, 2.0: 2, math.inf: 0}
+
+
+def _dense(t):
+    """Whether the elements of t fill one block of memory (in any order of its dimensions)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _clip(tensors, max_norm, norm_type, grad_scale, out):
+    """One call of snn_clip_grads: device tensor (2,) of the norm and the coefficient min(1, max_norm / (norm + 1e-6))."""
+    src = list(tensors)
+    try:
+        code = _NORM_TYPES[float(norm_type)]
+    except KeyError:
+        raise L.SnnError(f"norm_type {norm_type!r}: supported are 1, 2 and inf") from None
+    if not src:
+        raise L.SnnError("no gradients")
+    dev = src[0].device
+    if dev.type != "cuda":
+        raise L.SnnError("gradients must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")
+    try:
+        dts = [_DTYPES[t.dtype] for t in src]
+    except KeyError as e:
+        raise L.SnnError(f"gradients of type {e.args[0]}: supported are float32, bfloat16 and float16") from None
+    for t in src:
+        if t.device != dev or not (t.is_contiguous() or _dense(t)):
+            raise L.SnnError("gradients must be dense tensors (no gaps, no repeated elements) on one device")
+    n = len(src)
+    ptrs = [t.data_ptr() for t in src]
+    dst = None
+    if out is not None:
+        out = list(out)
+        full = [p for p, t in zip(ptrs, src) if t.numel()]
+        if len(set(full)) != len(full):
+            raise L.SnnError("a gradient is listed twice")
+        if len(out) != n:
+            raise L.SnnError(f"out has {len(out)} tensors for {n} gradients")
+        for t, o in zip(src, out):
+            if o is not t and (o.shape != t.shape or o.dtype != t.dtype or o.device != dev or
+                               (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))):
+                raise L.SnnError("out must match the gradients in shape, strides, type and device")
+        dst = (ctypes.c_void_p * n)(*[o.data_ptr() for o in out])
+    lib = L.load()
+    numel = (ctypes.c_int64 * n)(*[t.numel() for t in src])
+    doubles = L.check(lib.snn_clip_scratch_doubles(n, numel), "snn_clip_scratch_doubles")
+    with _on_device(dev):
+        buf = torch.empty(1 + doubles, dtype=torch.float64, device=dev)
+        p = buf.data_ptr()
+        L.check(lib.snn_clip_grads(n, (ctypes.c_void_p * n)(*ptrs), dst, numel, (ctypes.c_int32 * n)(*dts),
+                                   code, max_norm, grad_scale, p, p + 8, doubles, _stream()), "snn_clip_grads")
+    return buf[:1].view(torch.float32)
+
+
+def grad_norm(tensors, norm_type=2.0):
+    """The global norm (1, 2 or inf) of a list of dense fp32 / bf16 / fp16 device tensors, as a 0-dim fp32 device tensor
+    (no synchronisation).  Sums are fp64, in an order that depends on the sizes alone."""
+    return _clip(tensors, 1.0, norm_type, 1.0, None)[0]
+
+
+def clip_grads(tensors, max_norm, norm_type=2.0, out=None):
+    """Multiply every gradient by min(1, max_norm / (norm + 1e-6)), in place, or into `out` (a list of tensors like them);
+    returns the norm from before as a 0-dim fp32 device tensor.  Gradients that are not finite are not looked for: a norm of
+    inf gives 0 (and NaN where a gradient is inf), a norm of NaN gives NaN, as torch.nn.utils.clip_grad_norm_."""
+    tensors = list(tensors)
+    return _clip(tensors, float(max_norm), norm_type, 1.0, tensors if out is None else out)[0]
+
+
+def clip_coefficient(flat, max_norm, norm_type=2.0, grad_scale=1.0):
+    """(norm, coefficient) of grad_scale * flat as device tensor (2,), for adam_step / sgd_step's `clip`: the gradients
+    themselves are not touched, the update multiplies by the coefficient."""
+    return _clip([flat], float(max_norm), norm_type, grad_scale, None)
+
+
+def _check_clip(clip):
+    _require_cuda(clip, "clip")
+    if clip.numel() != 2:
+        raise L.SnnError("clip must be what clip_coefficient returned")
+    return ctypes.c_void_p(clip.data_ptr() + 4)
+
+
 def adam_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
-              grad_scale=1.0):
+              grad_scale=1.0, clip=None):
+    """`clip`: None, or clip_coefficient's (norm, coefficient): gradients are multiplied by grad_scale * coefficient."""
     for t, n in ((params, "params"), (grads, "grads"), (exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq")):
         _require_cuda(t, n)
         if t.numel() != params.numel():
             raise L.SnnError("adam_step: size mismatch")
+    if clip is not None:
+        L.check(L.load().snn_adam_step_clipped(params.numel(), _ptr(params), _ptr(grads), _ptr(exp_avg), _ptr(exp_avg_sq), step,
+                                               lr, betas[0], betas[1], eps, weight_decay, grad_scale, _check_clip(clip), _stream()),
+                "snn_adam_step_clipped")
+        return
     L.check(L.load().snn_adam_step(params.numel(), _ptr(params), _ptr(grads), _ptr(exp_avg), _ptr(exp_avg_sq), step,
                                    lr, betas[0], betas[1], eps, weight_decay, grad_scale, _stream()), "snn_adam_step")
 
 
-def sgd_step(params, grads, momentum_buf, step, lr, momentum=0.0, weight_decay=0.0, grad_scale=1.0):
+def sgd_step(params, grads, momentum_buf, step, lr, momentum=0.0, weight_decay=0.0, grad_scale=1.0, clip=None):
+    """`clip`: as adam_step."""
     for t, n in ((params, "params"), (grads, "grads"), (momentum_buf, "momentum_buf")):
         _require_cuda(t, n)
         if t.numel() != params.numel():
             raise L.SnnError("sgd_step: size mismatch")
+    if clip is not None:
+        L.check(L.load().snn_sgd_step_clipped(params.numel(), _ptr(params), _ptr(grads), _ptr(momentum_buf), step, lr, momentum,
+                                              weight_decay, grad_scale, _check_clip(clip), _stream()), "snn_sgd_step_clipped")
+        return
     L.check(L.load().snn_sgd_step(params.numel(), _ptr(params), _ptr(grads), _ptr(momentum_buf), step, lr, momentum,
                                   weight_decay, grad_scale, _stream()), "snn_sgd_step")

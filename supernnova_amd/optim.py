@@ -1,14 +1,35 @@
 """Fused optimizers over the module's flat parameter buffer (one kernel launch per step), with the
 data-parallel gradient all-reduce folded in.
   FusedAdam  torch.optim.Adam semantics (utils/training_utils.py:365-369): lr, betas (0.9, 0.999), eps 1e-8, L2 weight_decay
-  FusedSGD   torch.optim.SGD semantics with momentum (training/train_rnn.py:541-546, train_swag_finetune)"""
+  FusedSGD   torch.optim.SGD semantics with momentum (training/train_rnn.py:541-546, train_swag_finetune)
+Both clip by the global gradient norm when `max_grad_norm` is set: the norm is taken of the flat (all-reduced, averaged)
+gradient, and the update multiplies by the coefficient where it lies, on the device -- the gradient is read once more and
+never written.  clip_grad_norm_ does the same to the .grad tensors of any parameters, for other optimizers."""
 import torch
+
+from . import _lib as L
 
 from . import engine as E
 
 
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ over the gradients of `parameters` (a tensor or an iterable of them) with two launches of
+    hand-written kernels per 96 tensors and no synchronisation (error_if_nonfinite=True asks for one): returns the norm from
+    before as a 0-dim fp32 device tensor.  norm_type 1, 2 or inf."""
+    params = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    if error_if_nonfinite:
+        norm = E.grad_norm(grads, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise L.SnnError(f"the gradients' total norm of order {norm_type} is not finite: they cannot be clipped")
+    return E.clip_grads(grads, max_norm, norm_type)
+
+
 class _FlatOptimizer:
     _buffers = ()
+    last_grad_norm = None       # norm of the last step's gradient before clipping (0-dim device tensor; max_grad_norm set)
 
     def __init__(self, model, process_group=None, **hyper):
         self.model = model
@@ -62,8 +83,13 @@ class _FlatOptimizer:
         for k in self._buffers:
             if st[k] is None or st[k].numel() != flat.numel() or st[k].device != flat.device:
                 st[k] = torch.zeros_like(flat)
+        max_norm = self.param_groups[0].get("max_grad_norm")
+        clip = None
+        if max_norm is not None:
+            clip = E.clip_coefficient(grads, max_norm, grad_scale=scale)
+            self.last_grad_norm = clip[0]
         st["step"] += 1
-        self._update(flat, grads, scale)
+        self._update(flat, grads, scale, clip)
 
     def state_dict(self):
         return dict(state={k: (v.clone() if torch.is_tensor(v) else v) for k, v in self.state.items()},
@@ -77,21 +103,23 @@ class _FlatOptimizer:
 class FusedAdam(_FlatOptimizer):
     _buffers = ("exp_avg", "exp_avg_sq")
 
-    def __init__(self, model, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, process_group=None):
-        super().__init__(model, process_group, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+    def __init__(self, model, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, process_group=None,
+                 max_grad_norm=None):
+        super().__init__(model, process_group, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
 
-    def _update(self, flat, grads, scale):
+    def _update(self, flat, grads, scale, clip=None):
         g, st = self.param_groups[0], self.state
         E.adam_step(flat, grads, st["exp_avg"], st["exp_avg_sq"], st["step"], g["lr"], g["betas"], g["eps"],
-                    g["weight_decay"], scale)
+                    g["weight_decay"], scale, clip)
 
 
 class FusedSGD(_FlatOptimizer):
     _buffers = ("momentum_buffer",)
 
-    def __init__(self, model, lr=1e-3, momentum=0.0, weight_decay=0.0, process_group=None):
-        super().__init__(model, process_group, lr=lr, momentum=momentum, weight_decay=weight_decay)
+    def __init__(self, model, lr=1e-3, momentum=0.0, weight_decay=0.0, process_group=None, max_grad_norm=None):
+        super().__init__(model, process_group, lr=lr, momentum=momentum, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
 
-    def _update(self, flat, grads, scale):
+    def _update(self, flat, grads, scale, clip=None):
         g, st = self.param_groups[0], self.state
-        E.sgd_step(flat, grads, st["momentum_buffer"], st["step"], g["lr"], g["momentum"], g["weight_decay"], scale)
+        E.sgd_step(flat, grads, st["momentum_buffer"], st["step"], g["lr"], g["momentum"], g["weight_decay"], scale,
+                   clip)

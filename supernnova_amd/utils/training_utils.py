@@ -37,9 +37,11 @@ def get_model(settings, input_size):
 
 
 def get_optimizer(settings, model):
-    """Adam(lr, weight_decay) as training_utils.py:365-369 -- the fused HIP Adam over the flat buffer."""
+    """Adam(lr, weight_decay) as training_utils.py:365-369 -- the fused HIP Adam over the flat buffer.  `settings.max_grad_norm`,
+    where the settings have it (the reference's do not), clips by the global gradient norm."""
     from ..optim import FusedAdam
-    return FusedAdam(model, lr=settings.learning_rate, weight_decay=settings.weight_decay)
+    return FusedAdam(model, lr=settings.learning_rate, weight_decay=settings.weight_decay,
+                     max_grad_norm=getattr(settings, "max_grad_norm", None))
 
 
 def train_step(settings, rnn, packed_tensor, target_tensor, criterion, optimizer, batch_size, num_batches):
