@@ -51,15 +51,19 @@ template <int P> __device__ __forceinline__ double magnitude(float v, double a)
     if (P == 2) return fma((double)v, (double)v, a);
     return join<P>(a, (double)fabsf(v));
 }
-template <int P> __device__ __forceinline__ double block_join(double a)
+template <int P, int THREADS = 256> __device__ __forceinline__ double block_join(double a)
 {
-    __shared__ double s[4];
+    constexpr int WAVES = THREADS / 64;
+    __shared__ double s[WAVES];
 #pragma unroll
     for (int m = 32; m; m >>= 1) a = join<P>(a, __shfl_xor(a, m));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = a;
     __syncthreads();
-    return join<P>(join<P>(s[0], s[1]), join<P>(s[2], s[3]));
+    a = s[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) a = join<P>(a, s[w]);
+    return a;
 }
 template <typename T, int P> __device__ __forceinline__ double piece_sum(const T* g, int64_t n)
 {
@@ -97,19 +101,27 @@ template <int P> __global__ void __launch_bounds__(256) clip_norm_kernel(const T
     if (threadIdx.x == 0) part[blockIdx.x] = a;
 }
 // norm and coefficient from the pieces' sums, by one workgroup, always in the same order
-template <int P> __device__ __forceinline__ void finish(const double* part, int pieces, float max_norm, float grad_scale, float& norm, float& coef)
+template <int P, int THREADS> __device__ __forceinline__ void finish(const double* part, int pieces, float max_norm, float grad_scale, float& norm, float& coef)
 {
     double a = 0.0;
-    for (int i = threadIdx.x; i < pieces; i += 256) a = join<P>(a, part[i]);
-    a = block_join<P>(a);
+    int i = threadIdx.x;
+    for (; i + 7 * THREADS < pieces; i += 8 * THREADS) {          // eight loads in flight
+        double v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = part[i + u * THREADS];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) a = join<P>(a, v[u]);
+    }
+    for (; i < pieces; i += THREADS) a = join<P>(a, part[i]);
+    a = block_join<P, THREADS>(a);
     norm = (float)((double)grad_scale * (P == 2 ? sqrt(a) : a));
     coef = max_norm / (norm + 1e-6f);
     coef = coef > 1.0f ? 1.0f : coef;                          // a NaN stays
 }
-template <int P> __global__ void __launch_bounds__(256) clip_finish_kernel(const double* part, int pieces, float max_norm, float grad_scale, float* out)
+template <int P> __global__ void __launch_bounds__(1024) clip_finish_kernel(const double* part, int pieces, float max_norm, float grad_scale, float* out)
 {
     float norm, coef;
-    finish<P>(part, pieces, max_norm, grad_scale, norm, coef);
+    finish<P, 1024>(part, pieces, max_norm, grad_scale, norm, coef);
     if (threadIdx.x == 0) {
         out[0] = norm;
         out[1] = coef;
@@ -145,7 +157,7 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(const Table t, const do
 {
     float norm, c;
     if (DIRECT) {
-        finish<P>(part, pieces, max_norm, grad_scale, norm, c);
+        finish<P, 256>(part, pieces, max_norm, grad_scale, norm, c);
         if (write_out && blockIdx.x == 0 && threadIdx.x == 0) {
             out[0] = norm;
             out[1] = c;
@@ -228,7 +240,7 @@ void run(int n_tensors, const void* const* src, void* const* dst, const int64_t*
         hipLaunchKernelGGL((clip_norm_kernel<P>), dim3(here), w, 0, s, t, part + before);
     });
     const bool direct = dst && pieces && pieces <= CLIP_DIRECT;
-    if (!direct) hipLaunchKernelGGL((clip_finish_kernel<P>), dim3(1), w, 0, s, (const double*)part, (int)pieces, max_norm, grad_scale, out);
+    if (!direct) hipLaunchKernelGGL((clip_finish_kernel<P>), dim3(1), dim3(1024), 0, s, (const double*)part, (int)pieces, max_norm, grad_scale, out);
     if (dst)
         each_table(n_tensors, src, dst, numel, dtype, [&](const Table& t, int here, int64_t before) {
             if (direct)

@@ -222,23 +222,16 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
     }
 }
 
-// dweight (D, W) and dbias (D) from the slots' partial sums: 32 columns x 8 rows of threads, fp64, fixed order
-__global__ void __launch_bounds__(256) conv_bwd_sum_kernel(const float* __restrict__ part, int slots, int W, int D, float* dweight, float* dbias)
+// dweight (D, W) and dbias (D) from the slots' partial sums
+__global__ void __launch_bounds__(1024) conv_bwd_sum_kernel(const float* __restrict__ part, int slots, int W, int D, float* dweight, float* dbias)
 {
-    __shared__ double s[8][32];
-    const int n = (W + 1) * D, col = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
-    double a = 0.0;
-    if (col < n)
-        for (int i = row; i < slots; i += 8) a += part[(int64_t)i * n + col];
-    s[row][threadIdx.x & 31] = a;
-    __syncthreads();
-    if (row == 0 && col < n) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) a += s[i][threadIdx.x];
-        const int k = col / D, d = col - k * D;
-        if (k < W) dweight[(int64_t)d * W + k] = (float)a;
-        else if (dbias) dbias[d] = (float)a;
-    }
+    const int64_t n = (int64_t)(W + 1) * D;
+    int64_t col;
+    double a;
+    if (!column_sum(part, slots, n, n, &col, &a)) return;
+    const int k = (int)(col / D), d = (int)(col - (int64_t)k * D);
+    if (k < W) dweight[(int64_t)d * W + k] = (float)a;
+    else if (dbias) dbias[d] = (float)a;
 }
 
 template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_step_kernel(const ConvP<T> p)
@@ -349,7 +342,7 @@ template <typename T, int V, int W> int launch(const snn_conv_args* a, int what,
     }
     if constexpr (V <= 4) if (what == BWD) {
         hipLaunchKernelGGL((conv_bwd_kernel<T, V, W>), g, t, 0, s, p);
-        hipLaunchKernelGGL(conv_bwd_sum_kernel, dim3((unsigned)(((W + 1) * p.D + 31) / 32)), t, 0, s, (const float*)p.part, p.slots, W, p.D,
+        hipLaunchKernelGGL(conv_bwd_sum_kernel, dim3((unsigned)(((int64_t)(W + 1) * p.D + 15) / 16)), dim3(1024), 0, s, (const float*)p.part, p.slots, W, p.D,
                            a->dweight, a->dbias);
     }
     HIP_CHECK(hipGetLastError());

@@ -8,8 +8,8 @@
 // recomputes the segment's states and decays into registers (one exp per (step, channel, state), as the forward), then runs
 // the adjoint over it; neither is ever divided by a decay.  Sums over states are two DPP adds a quad, dealt over it; sums over
 // channels (dB, dC: 2K values a lane and step) are folded over the wave by v_permlane32_swap / v_permlane16_swap, each of which
-// halves the number of live values while it adds, then two DPP rotations, then LDS over the four waves, then -- layers wider than
-// 64 channels -- fp32 partial rows per channel block, added in order by scan_bc_sum_kernel.  Parameter gradients stay in registers over
+// halves the number of live values while it adds, then DPP rotations, then LDS over the four waves, then -- layers wider than
+// one workgroup's channels -- fp32 partial rows per channel block, added in order by scan_bc_sum_kernel.  Parameter gradients stay in registers over
 // all chunks a workgroup takes and are summed in fp64, in order, by scan_param_sum_kernel.  No atomics.
 #include <algorithm>
 #include "snn_host.h"
@@ -32,9 +32,9 @@ __device__ __forceinline__ void swap16(float& a, float& b)
     a = __uint_as_float(r[0]);
     b = __uint_as_float(r[1]);
 }
-// Sums over the wave's 16 channels (lanes of equal lane % 4) of b[0..K), c[0..K).  Row r = lane / 16 receives, for
-// i < K / 2, the sum of (r / 2 ? c : b)[i + (r % 2) K / 2], in all of its four quads.
-template <int K> __device__ __forceinline__ void channel_sums(float (&b)[K], float (&c)[K], float (&out)[K / 2])
+// Sums over the wave's 64 / LN channels (lanes of equal lane % LN) of b[0..K), c[0..K).  Row r = lane / 16 receives, for
+// i < K / 2, the sum of (r / 2 ? c : b)[i + (r % 2) K / 2], once for every channel of the row.
+template <int K, int LN> __device__ __forceinline__ void channel_sums(float (&b)[K], float (&c)[K], float (&out)[K / 2])
 {
 #pragma unroll
     for (int i = 0; i < K; ++i) {
@@ -45,115 +45,112 @@ template <int K> __device__ __forceinline__ void channel_sums(float (&b)[K], flo
     for (int i = 0; i < K / 2; ++i) {
         swap16(b[i], b[i + K / 2]);
         float v = b[i] + b[i + K / 2];
-        v += dpp<0x124>(v);                      // row_ror:4
-        out[i] = v + dpp<0x128>(v);              // row_ror:8
+        if constexpr (LN <= 4) v += dpp<0x124>(v);        // row_ror:4
+        if constexpr (LN <= 8) v += dpp<0x128>(v);        // row_ror:8
+        out[i] = v;
     }
 }
 
 // floats of one slot's parameter gradients: dA (D, 4K), dskip (D), dbias (D), and up to 16 bytes
 __host__ __device__ __forceinline__ int64_t part_stride(int D, int NP) { return ((int64_t)D * (NP + 2) + 3) / 4 * 4; }
 
-template <typename T, int G> struct BwdIn {
-    T x[G], d[G], z[G], y[G];
-    __device__ __forceinline__ void load(const ScanP<T>& p, int64_t xb, int64_t db, int64_t zb, int64_t gb, int t, int t1)
-    {
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-            if (t + 4 * i < t1) {
-                x[i] = p.x.p[xb + (t + 4 * i) * p.x.st];
-                d[i] = p.delta.p[db + (t + 4 * i) * p.delta.st];
-                if (p.z.p) z[i] = p.z.p[zb + (t + 4 * i) * p.z.st];
-                y[i] = p.dy.p[gb + (t + 4 * i) * p.dy.st];
-            }
-        }
-    }
-};
-
-template <int Q> __device__ __forceinline__ float qb(float v) { return quad_bcast<Q>(v); }
-__device__ __forceinline__ float qbc(float v, int q) { return q == 0 ? qb<0>(v) : q == 1 ? qb<1>(v) : q == 2 ? qb<2>(v) : qb<3>(v); }
-
 // What chunk c > 0 sends back from a zero adjoint, a_{t0} q_{t0}, into carry[b][c - 1], and the sum of its steps into csum[b][c].
-template <typename T, int K> __global__ void __launch_bounds__(256) scan_adjoint_kernel(const ScanP<T> p)
+template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds__(256) scan_adjoint_kernel(const ScanP<T> p)
 {
-    constexpr int SEG = SCAN_SEG, G = SEG / 4;
-    __shared__ float sC[2][SEG * 4 * K];
-    const int tid = threadIdx.x, nch = p.D / p.dg * p.cbg, cb = blockIdx.x % nch;
-    const int item = blockIdx.x / nch, b = item / p.nc, c = item - b * p.nc;
-    const ScanCh ch = scan_channel(cb, p.cbg, p.dg, tid);
+    constexpr int SEG = SCAN_SEG, G = SEG / 4, NP = K * LN;
+    __shared__ float sC[2][SEG * NP];
+    const int tid = threadIdx.x, b = blockIdx.x, cb = blockIdx.y, c = blockIdx.z;
+    const ScanCh ch = scan_channel<K, LN>(cb, p.cbg, p.dg, tid);
     const int j = ch.j, d = ch.d;
     const SeqRange r = seq_range(p.seq, b);
     const int t0 = c * p.tc, t1 = t0 + p.tc < r.len ? t0 + p.tc : r.len;
     if (c == 0 || t0 >= r.len) return;
-    const int64_t xb = r.row0 * p.x.st + b * p.x.sb + d, db = r.row0 * p.delta.st + b * p.delta.sb + d;
-    const int64_t zb = r.row0 * p.z.st + b * p.z.sb + d, gb = r.row0 * p.dy.st + b * p.dy.sb + d;
-    const T* Cp = p.C.p + r.row0 * p.C.st + b * p.C.sb + ch.g * p.C_sg;
     float w[K], A2[K];
-    load_states<K>(p.A + (int64_t)d * p.N, j, p.N, p.vec, A2);
+    load_states<K>(p.A + (int64_t)d * p.N, ch.n, p.N, p.vec, A2);
+    const float bias = p.dbias ? p.dbias[d] : 0.0f;
+    float ssum = 0.0f;
+    const int tl = t0 + (t1 - 1 - t0) / SEG * SEG;
+    const int64_t first = r.row0 + tl + j;               // pointers to the last segment; they move back with it
+    const T* dp = p.delta.p + first * p.delta.st + b * p.delta.sb + d;
+    const T* zp = GATE ? p.z.p + first * p.z.st + b * p.z.sb + d : nullptr;
+    const T* gp = p.dy.p + first * p.dy.st + b * p.dy.sb + d;
+    LaneIn<T, G> di, zi, gi;
+    RowStage<T, NP, SEG> Ci;
+    Ci.init(p.C.p + (r.row0 + tl) * p.C.st + b * p.C.sb + ch.g * p.C_sg, p.C.st, p.N, tid);
+    auto fetch = [&](int left) {
+        di.load(dp, p.delta.st, j, left);
+        if (GATE) zi.load(zp, p.z.st, j, left);
+        gi.load(gp, p.dy.st, j, left);
+        Ci.load(p.C.st, left);
+        dp -= SEG * p.delta.st;
+        if (GATE) zp -= SEG * p.z.st;
+        gp -= SEG * p.dy.st;
+        Ci.p -= SEG * p.C.st;
+    };
+    fetch(t1 - tl);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         A2[k] *= SNN_LOG2E;
         w[k] = 0.0f;
     }
-    const float bias = p.dbias ? p.dbias[d] : 0.0f;
-    float ssum = 0.0f;
-    BwdIn<T, G> in;
-    BcStage<T, K, SEG> bc;
-    const int tl = t0 + (t1 - 1 - t0) / SEG * SEG;
-    in.load(p, xb, db, zb, gb, tl + j, t1);
-    bc.template load<false>(Cp, p.C.st, Cp, p.C.st, tl, t1, p.N, tid);
     int buf = 0;
     for (int t = tl; t >= t0; t -= SEG, buf ^= 1) {
-        bc.template store<false>(sC[buf], nullptr, tid);
+        Ci.store(sC[buf], tid);
         float s[G], g[G];
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            const bool live = t + 4 * i + j < t1;
-            const float v = live ? to_f32(in.d[i]) + bias : 0.0f;
-            const float sp = p.softplus ? softplus_f32(v, nullptr) : v;
-            s[i] = live ? sp : 0.0f;
-            g[i] = live ? to_f32(in.y[i]) : 0.0f;
-            if (live && p.z.p) {
-                const float z = to_f32(in.z[i]);
+            const float v = to_f32(di.v[i]) + bias;
+            s[i] = p.softplus ? softplus_f32(v, nullptr) : v;
+            g[i] = to_f32(gi.v[i]);
+            if (GATE) {
+                const float z = to_f32(zi.v[i]);
                 g[i] *= z * sigmoid_f32(z);
             }
-            ssum += s[i];
+        }
+        if (t + SEG > t1) {
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                const bool live = t + 4 * i + j < t1;
+                s[i] = live ? s[i] : 0.0f;
+                g[i] = live ? g[i] : 0.0f;
+            }
         }
         __syncthreads();
-        if (t > t0) {
-            in.load(p, xb, db, zb, gb, t - SEG + j, t1);
-            bc.template load<false>(Cp, p.C.st, Cp, p.C.st, t - SEG, t1, p.N, tid);
-        }
+        if (t > t0) fetch(SEG);
+        float Cv[2][K];                                  // of this step and the next
+        lds_states<K>(&sC[buf][(SEG - 1) * NP], ch.n, Cv[1]);
 #pragma unroll
         for (int i = G - 1; i >= 0; --i) {
+            ssum += s[i];
 #pragma unroll
             for (int q = 3; q >= 0; --q) {
+                const int m = 4 * i + q;
+                if (m > 0) lds_states<K>(&sC[buf][(m - 1) * NP], ch.n, Cv[(m - 1) & 1]);
+                pin_lds_reads();
                 const float sq = qbc(s[i], q), gq = qbc(g[i], q);
-                float Cv[K];
-                lds_states<K>(&sC[buf][(4 * i + q) * 4 * K], j, Cv);
 #pragma unroll
-                for (int k = 0; k < K; ++k) w[k] = __builtin_amdgcn_exp2f(sq * A2[k]) * fmaf(Cv[k], gq, w[k]);
+                for (int k = 0; k < K; ++k) w[k] = __builtin_amdgcn_exp2f(sq * A2[k]) * fmaf(Cv[m & 1][k], gq, w[k]);
             }
         }
     }
     ssum = quad_sum(ssum);
     if (ch.ok) {
-        store_states<K>(p.carry + (((int64_t)b * p.nc + c - 1) * p.D + d) * (4 * K), j, 4 * K, true, w);
-        if (j == 0) p.csum[((int64_t)b * p.nc + c) * p.D + d] = ssum;
+        store_states<K>(p.carry + (((int64_t)b * p.nc + c - 1) * p.D + d) * NP, ch.n, NP, true, w);
+        if (ch.n == 0) p.csum[((int64_t)b * p.nc + c) * p.D + d] = ssum;
     }
 }
 
-template <typename T, int K> __global__ void __launch_bounds__(256, K == 16 ? 1 : 2) scan_bwd_kernel(const ScanP<T> p)
+template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds__(256, 2) scan_bwd_kernel(const ScanP<T> p)
 {
-    constexpr int SEG = ScanTape<K>::STEPS, G = SEG / 4, NP = 4 * K;
+    constexpr int SEG = ScanTape<K>::STEPS, G = SEG / 4, NP = K * LN, CH = 256 / LN;
     __shared__ float sB[2][SEG * NP], sC[2][SEG * NP], red[4][SEG][2 * NP];
     const int tid = threadIdx.x, nch = p.D / p.dg * p.cbg, cb = blockIdx.x % nch, slot = blockIdx.x / nch;
     const int wave = tid >> 6, lane = tid & 63;
-    const ScanCh ch = scan_channel(cb, p.cbg, p.dg, tid);
+    const ScanCh ch = scan_channel<K, LN>(cb, p.cbg, p.dg, tid);
     const int j = ch.j, d = ch.d;
-    const float live_ch = ch.ok ? 1.0f : 0.0f;
-    const int left = p.dg - (cb - ch.g * p.cbg) * SCAN_CH, d0 = ch.g * p.dg + p.dg - left;
+    const int left_ch = p.dg - (cb - ch.g * p.cbg) * CH, d0 = ch.g * p.dg + p.dg - left_ch;
     float A2[K], dA[K], dsk = 0.0f, dbs = 0.0f;
-    load_states<K>(p.A + (int64_t)d * p.N, j, p.N, p.vec, A2);
+    load_states<K>(p.A + (int64_t)d * p.N, ch.n, p.N, p.vec, A2);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         A2[k] *= SNN_LOG2E;
@@ -167,84 +164,109 @@ template <typename T, int K> __global__ void __launch_bounds__(256, K == 16 ? 1 
         const int b = item / p.nc, c = item - b * p.nc;
         const SeqRange r = seq_range(p.seq, b);
         const int t0 = c * p.tc, t1 = t0 + p.tc < r.len ? t0 + p.tc : r.len;
-        const int64_t xb = r.row0 * p.x.st + b * p.x.sb + d, db = r.row0 * p.delta.st + b * p.delta.sb + d;
-        const int64_t zb = r.row0 * p.z.st + b * p.z.sb + d, gb = r.row0 * p.dy.st + b * p.dy.sb + d;
-        const int64_t dxb = r.row0 * p.dx.st + b * p.dx.sb, ddb = r.row0 * p.ddelta.st + b * p.ddelta.sb;
-        const int64_t dzb = r.row0 * p.dz.st + b * p.dz.sb;
-        const int64_t dBb = r.row0 * p.dB.st + b * p.dB.sb + ch.g * p.N, dCb = r.row0 * p.dC.st + b * p.dC.sb + ch.g * p.N;
         const int64_t rowb = p.seq.offsets ? r.row0 : (int64_t)b * p.seq.max_T;
-        const T* Bp = p.B.p + r.row0 * p.B.st + b * p.B.sb + ch.g * p.B_sg;
-        const T* Cp = p.C.p + r.row0 * p.C.st + b * p.C.sb + ch.g * p.C_sg;
         float w[K];                                               // a_{t+1} q_{t+1}
 #pragma unroll
         for (int k = 0; k < K; ++k) w[k] = 0.0f;
-        if (p.nc > 1 && t0 < r.len) load_states<K>(p.carry + (((int64_t)b * p.nc + c) * p.D + d) * NP, j, NP, true, w);
-        else if (c == 0 && p.dhT) load_states<K>(p.dhT + ((int64_t)b * p.D + d) * p.N, j, p.N, p.vec, w);
+        if (p.nc > 1 && t0 < r.len) load_states<K>(p.carry + (((int64_t)b * p.nc + c) * p.D + d) * NP, ch.n, NP, true, w);
+        else if (c == 0 && p.dhT) load_states<K>(p.dhT + ((int64_t)b * p.D + d) * p.N, ch.n, p.N, p.vec, w);
         if (t0 < t1) {
-            BwdIn<T, G> in;
-            BcStage<T, K, SEG> bc;
-            float hs[K];
             const int tl = t0 + (t1 - 1 - t0) / SEG * SEG;
-            const float* tape = p.tape + ((scan_tape_first(p.seq, r, b, SEG) + tl / SEG) * p.D + d) * NP;
-            in.load(p, xb, db, zb, gb, tl + j, t1);
-            bc.template load<true>(Bp, p.B.st, Cp, p.C.st, tl, t1, p.N, tid);
-            load_states<K>(tape, j, NP, true, hs);
+            const int64_t first = r.row0 + tl + j;       // pointers to the last segment; they move back with it
+            const T* xp = p.x.p + first * p.x.st + b * p.x.sb + d;
+            const T* dp = p.delta.p + first * p.delta.st + b * p.delta.sb + d;
+            const T* zp = GATE ? p.z.p + first * p.z.st + b * p.z.sb + d : nullptr;
+            const T* gp = p.dy.p + first * p.dy.st + b * p.dy.sb + d;
+            T* dxp = p.dx.p + first * p.dx.st + b * p.dx.sb + d;
+            T* ddp = p.ddelta.p + first * p.ddelta.st + b * p.ddelta.sb + d;
+            T* dzp = GATE ? p.dz.p + first * p.dz.st + b * p.dz.sb + d : nullptr;
+            const float* tape = p.tape + ((scan_tape_first(p.seq, r, b, SEG) + tl / SEG) * p.D + d) * NP + ch.n;
+            LaneIn<T, G> xi, di, zi, gi;
+            RowStage<T, NP, SEG> Bi, Ci;
+            Bi.init(p.B.p + (r.row0 + tl) * p.B.st + b * p.B.sb + ch.g * p.B_sg, p.B.st, p.N, tid);
+            Ci.init(p.C.p + (r.row0 + tl) * p.C.st + b * p.C.sb + ch.g * p.C_sg, p.C.st, p.N, tid);
+            float hs[K];
+            auto fetch = [&](int left) {
+                xi.load(xp, p.x.st, j, left);
+                di.load(dp, p.delta.st, j, left);
+                if (GATE) zi.load(zp, p.z.st, j, left);
+                gi.load(gp, p.dy.st, j, left);
+                Bi.load(p.B.st, left);
+                Ci.load(p.C.st, left);
+                load_states<K>(tape, 0, NP, true, hs);
+                xp -= SEG * p.x.st;
+                dp -= SEG * p.delta.st;
+                if (GATE) zp -= SEG * p.z.st;
+                gp -= SEG * p.dy.st;
+                Bi.p -= SEG * p.B.st;
+                Ci.p -= SEG * p.C.st;
+                tape -= (int64_t)p.D * NP;
+            };
+            fetch(t1 - tl);
             int buf = 0;
             for (int t = tl; t >= t0; t -= SEG, buf ^= 1) {
-                bc.template store<true>(sB[buf], sC[buf], tid);
+                Bi.store(sB[buf], tid);
+                Ci.store(sC[buf], tid);
                 float x[G], s[G], sig[G], z[G], dy[G], g[G], u[G], h[SEG + 1][K], a[SEG][K];
 #pragma unroll
                 for (int i = 0; i < G; ++i) {
-                    const bool live = t + 4 * i + j < t1;
-                    const float lc = live ? live_ch : 0.0f;       // lanes without a channel must add nothing to dB, dC
-                    x[i] = live ? to_f32(in.x[i]) : 0.0f;
-                    const float v = live ? to_f32(in.d[i]) + bias : 0.0f;
-                    float sp = v;
+                    x[i] = to_f32(xi.v[i]);
+                    const float v = to_f32(di.v[i]) + bias;
+                    s[i] = v;
                     sig[i] = 1.0f;
-                    if (p.softplus) sp = softplus_f32(v, &sig[i]);
-                    s[i] = live ? sp : 0.0f;
-                    z[i] = live && p.z.p ? to_f32(in.z[i]) : 0.0f;
-                    dy[i] = live && lc != 0.0f ? to_f32(in.y[i]) : 0.0f;
-                    g[i] = p.z.p ? dy[i] * z[i] * sigmoid_f32(z[i]) : dy[i];
-                    u[i] = lc != 0.0f ? s[i] * x[i] : 0.0f;
+                    if (p.softplus) s[i] = softplus_f32(v, &sig[i]);
+                    dy[i] = to_f32(gi.v[i]);
+                    z[i] = GATE ? to_f32(zi.v[i]) : 0.0f;
+                }
+                const int left = t1 - t;
+                if (left < SEG || left_ch < CH) {        // steps behind the end leave the state, lanes without a channel add nothing
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        const bool live = 4 * i + j < left;
+                        s[i] = live ? s[i] : 0.0f;
+                        x[i] = live && ch.ok ? x[i] : 0.0f;
+                        dy[i] = live && ch.ok ? dy[i] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    u[i] = s[i] * x[i];
+                    g[i] = GATE ? dy[i] * (z[i] * sigmoid_f32(z[i])) : dy[i];
                 }
 #pragma unroll
                 for (int k = 0; k < K; ++k) h[0][k] = hs[k];
                 __syncthreads();              // B, C staged; the last segment's partial sums have been read
-                if (t > t0) {
-                    in.load(p, xb, db, zb, gb, t - SEG + j, t1);
-                    bc.template load<true>(Bp, p.B.st, Cp, p.C.st, t - SEG, t1, p.N, tid);
-                    tape -= (int64_t)p.D * NP;
-                    load_states<K>(tape, j, NP, true, hs);
-                }
+                if (t > t0) fetch(SEG);
                 // the segment's states and decays again
+                float Bv[2][K], Cv[2][K];                // of this step and the next
+                auto read = [&](int m, bool want_c) {
+                    lds_states<K>(&sB[buf][m * NP], ch.n, Bv[m & 1]);
+                    if (want_c) lds_states<K>(&sC[buf][m * NP], ch.n, Cv[m & 1]);
+                };
+                read(0, GATE);
 #pragma unroll
                 for (int i = 0; i < G; ++i) {
-                    float yp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float yv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
+                        const int m = 4 * i + q;
+                        if (m + 1 < SEG) read(m + 1, GATE);
+                        pin_lds_reads();
                         const float sq = qbc(s[i], q), uq = qbc(u[i], q);
-                        float Bv[K];
-                        lds_states<K>(&sB[buf][(4 * i + q) * NP], j, Bv);
 #pragma unroll
                         for (int k = 0; k < K; ++k) {
-                            a[4 * i + q][k] = __builtin_amdgcn_exp2f(sq * A2[k]);
-                            h[4 * i + q + 1][k] = fmaf(a[4 * i + q][k], h[4 * i + q][k], uq * Bv[k]);
-                        }
-                        if (p.z.p) {
-                            float Cv[K];
-                            lds_states<K>(&sC[buf][(4 * i + q) * NP], j, Cv);
-#pragma unroll
-                            for (int k = 0; k < K; ++k) yp[q] = fmaf(h[4 * i + q + 1][k], Cv[k], yp[q]);
+                            a[m][k] = __builtin_amdgcn_exp2f(sq * A2[k]);
+                            h[m + 1][k] = fmaf(a[m][k], h[m][k], uq * Bv[m & 1][k]);
+                            if (GATE) yv[q] = fmaf(h[m + 1][k], Cv[m & 1][k], yv[q]);
                         }
                     }
-                    if (p.z.p) {
-                        const float y = fmaf(skip, x[i], quad_reduce_scatter(yp, j)), e = sigmoid_f32(z[i]);
-                        const int tt = t + 4 * i + j;
-                        if (ch.ok && tt < t1) p.dz.p[dzb + tt * p.dz.st + d] = from_f32<T>(dy[i] * y * (e * fmaf(z[i], 1.0f - e, 1.0f)));
+                    if (GATE) {
+                        const float y = fmaf(skip, x[i], step_sums<LN>(yv, j)), e = sigmoid_f32(z[i]);
+                        if (ch.lead && 4 * i + j < left) dzp[4 * i * p.dz.st] = from_f32<T>(dy[i] * y * (e * fmaf(z[i], 1.0f - e, 1.0f)));
                     }
                 }
                 // the adjoint, backwards
+                read(SEG - 1, true);
 #pragma unroll
                 for (int i = G - 1; i >= 0; --i) {
                     float s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -252,121 +274,129 @@ template <typename T, int K> __global__ void __launch_bounds__(256, K == 16 ? 1 
                     for (int q = 3; q >= 0; --q) {
                         const int m = 4 * i + q;
                         const float sq = qbc(s[i], q), uq = qbc(u[i], q), gq = qbc(g[i], q);
-                        float Bv[K], Cv[K], pb[K], pc[K], sums[K / 2];
-                        lds_states<K>(&sB[buf][m * NP], j, Bv);
-                        lds_states<K>(&sC[buf][m * NP], j, Cv);
+                        if (m > 0) read(m - 1, true);
+                        pin_lds_reads();
+                        float pb[K], pc[K], sums[K / 2];
 #pragma unroll
                         for (int k = 0; k < K; ++k) {
-                            const float qk = fmaf(Cv[k], gq, w[k]);
+                            const float qk = fmaf(Cv[m & 1][k], gq, w[k]);
                             pc[k] = gq * h[m + 1][k];
                             pb[k] = qk * uq;
-                            s1[q] = fmaf(qk, Bv[k], s1[q]);
+                            s1[q] = fmaf(qk, Bv[m & 1][k], s1[q]);
                             w[k] = a[m][k] * qk;
                             const float v = w[k] * h[m][k];
                             dA[k] = fmaf(v, sq, dA[k]);
                             s2[q] = fmaf(v, A2[k], s2[q]);
                         }
-                        channel_sums<K>(pb, pc, sums);
-                        if ((lane & 12) == 0) {
-                            float* o = &red[wave][m][(lane >> 5) * NP + j * K + ((lane >> 4) & 1) * (K / 2)];
+                        channel_sums<K, LN>(pb, pc, sums);
+                        if ((lane & 15) < LN) {
+                            float* o = &red[wave][m][(lane >> 5) * NP + ch.n + ((lane >> 4) & 1) * (K / 2)];
 #pragma unroll
                             for (int k = 0; k < K / 2; ++k) o[k] = sums[k];
                         }
                     }
-                    const float qB = quad_reduce_scatter(s1, j), wA = quad_reduce_scatter(s2, j) * SNN_LN2;
-                    const int tt = t + 4 * i + j;
+                    const float qB = step_sums<LN>(s1, j), wA = step_sums<LN>(s2, j) * SNN_LN2;
                     const float dd = fmaf(x[i], qB, wA) * sig[i];
-                    if (ch.ok && tt < t1) {
-                        p.dx.p[dxb + tt * p.dx.st + d] = from_f32<T>(fmaf(skip, g[i], s[i] * qB));
-                        p.ddelta.p[ddb + tt * p.ddelta.st + d] = from_f32<T>(dd);
+                    if (ch.lead && 4 * i + j < left) {
+                        dxp[4 * i * p.dx.st] = from_f32<T>(fmaf(skip, g[i], s[i] * qB));
+                        ddp[4 * i * p.ddelta.st] = from_f32<T>(dd);
                         dbs += dd;
                         dsk = fmaf(g[i], x[i], dsk);
                     }
                 }
+                dxp -= SEG * p.dx.st;
+                ddp -= SEG * p.ddelta.st;
+                if (GATE) dzp -= SEG * p.dz.st;
                 __syncthreads();
                 for (int e = tid; e < SEG * 2 * NP; e += 256) {
-                    const int m = e / (2 * NP), o = e % (2 * NP), half = o / NP, n = o % NP, tt = t + m;
-                    if (tt < t1) {
+                    const int m = e / (2 * NP), o = e % (2 * NP), half = o / NP, n = o % NP;
+                    if (m < left) {
                         const float v = (red[0][m][o] + red[1][m][o]) + (red[2][m][o] + red[3][m][o]);
-                        if (bcpart) bcpart[(rowb + tt) * (2 * NP) + o] = v;
+                        if (bcpart) bcpart[(rowb + t + m) * (2 * NP) + o] = v;
                         else if (n < p.N) {
-                            if (half) p.dC.p[dCb + tt * p.dC.st + n] = from_f32<T>(v);
-                            else p.dB.p[dBb + tt * p.dB.st + n] = from_f32<T>(v);
+                            const View<T>& q = half ? p.dC : p.dB;
+                            q.p[(r.row0 + t + m) * q.st + b * q.sb + ch.g * p.N + n] = from_f32<T>(v);
                         }
                     }
                 }
             }
             __syncthreads();                  // the next chunk stages into the buffers this one has read
         }
-        if (c == 0 && p.dh0 && ch.ok) store_states<K>(p.dh0 + ((int64_t)b * p.D + d) * p.N, j, p.N, p.vec, w);
+        if (c == 0 && p.dh0 && ch.ok) store_states<K>(p.dh0 + ((int64_t)b * p.D + d) * p.N, ch.n, p.N, p.vec, w);
         const FillRange f = fill_range(p.seq, r, b, t0, t0 + p.tc, c == p.nc - 1);
-        const int n = left < SCAN_CH ? left : SCAN_CH;
-        clear_channels(p.dx, dxb, f, d0, n, tid);
-        clear_channels(p.ddelta, ddb, f, d0, n, tid);
-        if (p.dz.p) clear_channels(p.dz, dzb, f, d0, n, tid);
-        if (bcpart) {
+        const int n = left_ch < CH ? left_ch : CH;
+        clear_channels(p.dx, r.row0 * p.dx.st + b * p.dx.sb, f, d0, n, tid);
+        clear_channels(p.ddelta, r.row0 * p.ddelta.st + b * p.ddelta.sb, f, d0, n, tid);
+        if (GATE) clear_channels(p.dz, r.row0 * p.dz.st + b * p.dz.sb, f, d0, n, tid);
+        if (bcpart && p.seq.offsets) {
             for (int64_t e = f.a0 * (2 * NP) + tid; e < f.a1 * (2 * NP); e += 256) bcpart[rowb * (2 * NP) + e] = 0.0f;
             for (int64_t e = f.b0 * (2 * NP) + tid; e < f.b1 * (2 * NP); e += 256) bcpart[rowb * (2 * NP) + e] = 0.0f;
-        } else {
-            clear_channels(p.dB, dBb, f, 0, p.N, tid);
-            clear_channels(p.dC, dCb, f, 0, p.N, tid);
+        } else if (!bcpart) {
+            clear_channels(p.dB, r.row0 * p.dB.st + b * p.dB.sb + ch.g * p.N, f, 0, p.N, tid);
+            clear_channels(p.dC, r.row0 * p.dC.st + b * p.dC.sb + ch.g * p.N, f, 0, p.N, tid);
         }
     }
     dsk = quad_sum(dsk);
     dbs = quad_sum(dbs);
     if (ch.ok) {
         float* q = p.part + (int64_t)slot * part_stride(p.D, NP);
-        store_states<K>(q + (int64_t)d * NP, j, NP, true, dA);
-        if (j == 0) {
+        store_states<K>(q + (int64_t)d * NP, ch.n, NP, true, dA);
+        if (ch.n == 0) {
             q[(int64_t)p.D * NP + d] = dsk;
             q[(int64_t)p.D * (NP + 1) + d] = dbs;
         }
     }
 }
 
-// dA (D, N), dskip (D), dbias (D) from the slots' partial sums: 32 columns x 8 rows of threads, fp64, fixed order
-__global__ void __launch_bounds__(256) scan_param_sum_kernel(const float* __restrict__ part, int slots, int D, int N, int NP, float* dA, float* dskip,
+// dA (D, N), dskip (D), dbias (D) from the slots' partial sums
+__global__ void __launch_bounds__(1024) scan_param_sum_kernel(const float* __restrict__ part, int slots, int D, int N, int NP, float* dA, float* dskip,
                                                              float* dbias)
 {
-    __shared__ double s[8][32];
-    const int64_t n = (int64_t)D * (NP + 2), stride = part_stride(D, NP), col = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int row = threadIdx.x >> 5;
-    double a = 0.0;
-    if (col < n)
-        for (int i = row; i < slots; i += 8) a += part[(int64_t)i * stride + col];
-    s[row][threadIdx.x & 31] = a;
-    __syncthreads();
-    if (row == 0 && col < n) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) a += s[i][threadIdx.x];
-        if (col < (int64_t)D * NP) {
-            const int d = (int)(col / NP), k = (int)(col - (int64_t)d * NP);
-            if (k < N) dA[(int64_t)d * N + k] = (float)a;
-        } else if (col < (int64_t)D * (NP + 1)) {
-            if (dskip) dskip[col - (int64_t)D * NP] = (float)a;
-        } else if (dbias) dbias[col - (int64_t)D * (NP + 1)] = (float)a;
-    }
+    int64_t col;
+    double a;
+    if (!column_sum(part, slots, part_stride(D, NP), (int64_t)D * (NP + 2), &col, &a)) return;
+    if (col < (int64_t)D * NP) {
+        const int d = (int)(col / NP), k = (int)(col - (int64_t)d * NP);
+        if (k < N) dA[(int64_t)d * N + k] = (float)a;
+    } else if (col < (int64_t)D * (NP + 1)) {
+        if (dskip) dskip[col - (int64_t)D * NP] = (float)a;
+    } else if (dbias) dbias[col - (int64_t)D * (NP + 1)] = (float)a;
 }
 
-// dB, dC rows from the channel blocks' partial rows (cleared rows included), in block order
+// dB, dC rows from the channel blocks' partial rows, in block order, four states a thread.  In a padded batch the rows behind a
+// sequence's end are recognised here and never written as partial rows; among ragged rows they have been cleared.
 template <typename T> __global__ void __launch_bounds__(256) scan_bc_sum_kernel(const ScanP<T> p, int NP, int groups)
 {
-    const int64_t rows = p.seq.offsets ? p.seq.n_rows : (int64_t)p.seq.n_seq * p.seq.max_T, per = (int64_t)groups * 2 * NP;
+    const int64_t rows = p.seq.offsets ? p.seq.n_rows : (int64_t)p.seq.n_seq * p.seq.max_T;
+    const int quads = NP / 2, per = groups * quads;                 // of a group's 2 NP partial sums
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= rows * per) return;
     const int64_t row = id / per;
-    const int e = (int)(id - row * per), g = e / (2 * NP), o = e - g * 2 * NP, half = o / NP, n = o - half * NP;
-    if (n >= p.N) return;
-    const float* q = p.bcpart + ((int64_t)g * p.cbg * rows + row) * (2 * NP) + o;
-    float a = 0.0f;
-    for (int i = 0; i < p.cbg; ++i) a += q[(int64_t)i * rows * (2 * NP)];
+    const int e = (int)(id - row * per), g = e / quads, o = (e - g * quads) * 4, half = o >= NP, n = o - half * NP;
     int64_t t = row, b = 0;
+    bool live = true;
     if (!p.seq.offsets) {
         b = row / p.seq.max_T;
         t = row - b * p.seq.max_T;
+        live = t < seq_range(p.seq, (int)b).len;
     }
-    if (half) p.dC.p[t * p.dC.st + b * p.dC.sb + g * p.N + n] = from_f32<T>(a);
-    else p.dB.p[t * p.dB.st + b * p.dB.sb + g * p.N + n] = from_f32<T>(a);
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (live) {
+        const float* q = p.bcpart + ((int64_t)g * p.cbg * rows + row) * (2 * NP) + o;
+        for (int i = 0; i < p.cbg; ++i, q += rows * (2 * NP)) {
+            const float4 v = *(const float4*)q;
+            a.x += v.x;
+            a.y += v.y;
+            a.z += v.z;
+            a.w += v.w;
+        }
+    }
+    const View<T>& w = half ? p.dC : p.dB;
+    T* out = w.p + t * w.st + b * w.sb + g * p.N + n;
+    const float v[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < p.N) out[i] = from_f32<T>(v[i]);
 }
 
 struct Sizes { int64_t carry, csum, part, bc; int slots; };
@@ -374,7 +404,7 @@ struct Sizes { int64_t carry, csum, part, bc; int slots; };
 // ragged lengths; more would only add partial sums to write and read.
 Sizes sizes(const snn_scan_args* a, const ScanGrid& g)
 {
-    const int NP = 4 * scan_k(a->states);
+    const int NP = scan_padded(a->states);
     const int64_t items = (int64_t)a->seq.n_seq * g.nc;
     Sizes z;
     z.slots = (int)std::min<int64_t>(items, std::max<int64_t>(1, 2048 / g.blocks_c));
@@ -386,7 +416,7 @@ Sizes sizes(const snn_scan_args* a, const ScanGrid& g)
     return z;
 }
 
-template <typename T, int K> int backward(const snn_scan_args* a, const ScanGrid& g, hipStream_t s)
+template <typename T, int K, int LN, bool GATE> int backward(const snn_scan_args* a, const ScanGrid& g, hipStream_t s)
 {
     ScanP<T> p = scan_params<T>(a, g);
     const Sizes z = sizes(a, g);
@@ -395,31 +425,34 @@ template <typename T, int K> int backward(const snn_scan_args* a, const ScanGrid
     p.part = p.csum + z.csum;
     p.bcpart = z.bc ? p.part + z.part : nullptr;
     p.slots = z.slots;
-    const int64_t blocks = (int64_t)g.blocks_c * a->seq.n_seq * g.nc;
     if (g.nc > 1) {
-        hipLaunchKernelGGL((scan_adjoint_kernel<T, K>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+        const dim3 grid((unsigned)a->seq.n_seq, (unsigned)g.blocks_c, (unsigned)g.nc);
+        hipLaunchKernelGGL((scan_adjoint_kernel<T, K, LN, GATE>), grid, dim3(256), 0, s, p);
         snn_scan_launch_combine(a, g, a->dstate_out, p.carry, p.csum, true, s);
     }
-    hipLaunchKernelGGL((scan_bwd_kernel<T, K>), dim3((unsigned)(g.blocks_c * z.slots)), dim3(256), 0, s, p);
-    const int64_t n = (int64_t)p.D * (4 * K + 2);
-    hipLaunchKernelGGL(scan_param_sum_kernel, dim3((unsigned)((n + 31) / 32)), dim3(256), 0, s, (const float*)p.part, z.slots, p.D, p.N, 4 * K,
+    hipLaunchKernelGGL((scan_bwd_kernel<T, K, LN, GATE>), dim3((unsigned)(g.blocks_c * z.slots)), dim3(256), 0, s, p);
+    const int64_t n = (int64_t)p.D * (K * LN + 2);
+    hipLaunchKernelGGL(scan_param_sum_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, s, (const float*)p.part, z.slots, p.D, p.N, K * LN,
                        a->dA, a->dskip, a->ddelta_bias);
     if (z.bc) {
         const int64_t rows = a->seq.offsets ? a->seq.n_rows : (int64_t)a->seq.n_seq * a->seq.max_T;
-        const int64_t e = (rows * a->groups * 8 * K + 255) / 256;
-        hipLaunchKernelGGL((scan_bc_sum_kernel<T>), dim3((unsigned)e), dim3(256), 0, s, p, 4 * K, a->groups);
+        const int64_t e = (rows * a->groups * (K * LN / 2) + 255) / 256;
+        hipLaunchKernelGGL((scan_bc_sum_kernel<T>), dim3((unsigned)e), dim3(256), 0, s, p, K * LN, a->groups);
     }
     HIP_CHECK(hipGetLastError());
     return SNN_OK;
 }
+template <typename T, bool GATE> int by_states(const snn_scan_args* a, const ScanGrid& g, hipStream_t s)
+{
+    if (a->states <= 8) return backward<T, 2, 4, GATE>(a, g, s);
+    if (a->states <= 16) return backward<T, 4, 4, GATE>(a, g, s);
+    if (a->states <= 32) return backward<T, 4, 8, GATE>(a, g, s);
+    return backward<T, 4, 16, GATE>(a, g, s);
+}
+
 template <typename T> int run(const snn_scan_args* a, const ScanGrid& g, hipStream_t s)
 {
-    switch (scan_k(a->states)) {
-    case 2: return backward<T, 2>(a, g, s);
-    case 4: return backward<T, 4>(a, g, s);
-    case 8: return backward<T, 8>(a, g, s);
-    default: return backward<T, 16>(a, g, s);
-    }
+    return a->z.p ? by_states<T, true>(a, g, s) : by_states<T, false>(a, g, s);
 }
 
 }  // namespace
@@ -427,7 +460,7 @@ template <typename T> int run(const snn_scan_args* a, const ScanGrid& g, hipStre
 extern "C" int64_t snn_scan_workspace_bytes(const snn_scan_args* a, int32_t backward_pass)
 {
     if (int rc = snn_scan_check(a, "snn_scan_workspace_bytes")) return rc;
-    const ScanGrid g = snn_scan_grid(a, backward_pass != 0);
+    const ScanGrid g = snn_scan_grid(a);
     const Sizes z = sizes(a, g);
     return 4 * (z.carry + z.csum + (backward_pass ? z.part + z.bc : 0));
 }
@@ -446,9 +479,9 @@ extern "C" int snn_scan_backward(const snn_scan_args* a, void* stream)
                       (long long)need, (long long)a->tape_floats);
         return SNN_ERR_WORKSPACE;
     }
-    const ScanGrid g = snn_scan_grid(a, true);
+    const ScanGrid g = snn_scan_grid(a);
     const int64_t rows = a->seq.offsets ? a->seq.n_rows : (int64_t)a->seq.n_seq * a->seq.max_T;
-    if ((int64_t)g.blocks_c * a->seq.n_seq * g.nc > 0x7fffffff || (rows * a->groups * 8 * scan_k(a->states) + 255) / 256 > 0x7fffffff) {
+    if ((int64_t)a->seq.n_seq * g.nc > 0x7fffffff || (rows * a->groups * 2 * scan_padded(a->states) + 255) / 256 > 0x7fffffff) {
         snn_set_error("snn_scan_backward: grid too large");
         return SNN_ERR_UNSUPPORTED;
     }

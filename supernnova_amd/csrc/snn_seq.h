@@ -87,27 +87,51 @@ __device__ __forceinline__ float quad_reduce_scatter(const float v[4], int j)
 // ---- activations --------------------------------------------------------------------------------------------------
 #define SNN_LOG2E 1.44269504088896341f
 #define SNN_LN2 0.693147180559945309f
-// exp(v) to about an ulp: the product v * log2(e) is carried with its rounding error (|v| * 6e-8 of the result otherwise)
-__device__ __forceinline__ float exp_f32(float v)
-{
-    const float hi = v * SNN_LOG2E;
-    const float lo = fmaf(v, SNN_LOG2E, -hi) + v * 1.925963033500011e-08f;
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return fabsf(hi) < 150.0f ? fmaf(e, lo * SNN_LN2, e) : e;          // infinite products have no rounding error to add
-}
-__device__ __forceinline__ float sigmoid_f32(float v) { return __builtin_amdgcn_rcpf(1.0f + exp_f32(-v)); }
-// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) <= 1, and its derivative sigmoid(v).  log1p(e) = 2 atanh(s) with
-// s = e / (2 + e) <= 1/3: seven terms of the odd series leave 1.4e-8 of the first, below fp32 rounding for every v.
+// silu and its slope take 2^(-v log2 e) as it comes: an error of |v| 6e-8 in the exponential, at most 2e-8 |v| in the sigmoid
+__device__ __forceinline__ float sigmoid_f32(float v) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -SNN_LOG2E)); }
+// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) <= 1, and its derivative sigmoid(v).  Steps are small (v about -5), where
+// log1p(e) ~ e, so e has to be relatively exact: the rounding error of |v| log2(e) is put back, and log1p(e) is
+// log(u) + (e - (u - 1)), u = fl(1 + e): the second term is what the sum 1 + e dropped.
 __device__ __forceinline__ float softplus_f32(float v, float* sigma)
 {
-    const float e = exp_f32(-fabsf(v));
-    const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
-    float p = fmaf(q, 1.0f / 13, 1.0f / 11);
-    p = fmaf(q, p, 1.0f / 9);
-    p = fmaf(q, p, 1.0f / 7);
-    p = fmaf(q, p, 1.0f / 5);
-    p = fmaf(q, p, 1.0f / 3);
-    p = fmaf(q, p, 1.0f);
-    if (sigma) *sigma = (v >= 0.0f ? 1.0f : e) * __builtin_amdgcn_rcpf(1.0f + e);
-    return (v > 0.0f ? v : (v == v ? 0.0f : v)) + 2.0f * s * p;
+    const float w = fminf(fabsf(v), 104.0f);                       // exp(-104) = 0
+    const float hi = w * -SNN_LOG2E, lo = fmaf(w, -SNN_LOG2E, -hi);
+    const float e0 = __builtin_amdgcn_exp2f(hi), e = fmaf(e0, lo * SNN_LN2, e0);
+    const float u = 1.0f + e;
+    const float l = fmaf(__builtin_amdgcn_logf(u), SNN_LN2, e - (u - 1.0f));     // v_log_f32: base 2
+    if (sigma) *sigma = (v >= 0.0f ? 1.0f : e) * __builtin_amdgcn_rcpf(u);
+    return (v <= 0.0f ? 0.0f : v) + l;                             // not v > 0: a NaN stays
+}
+
+// ---- sums over workgroups -----------------------------------------------------------------------------------------
+// Column `col` of part[slots][stride] in fp64 and in an order that depends on `slots` alone: a workgroup of 1024 threads sums 16
+// columns, 64 rows at a time.  True for the 16 threads that receive a sum.
+__device__ __forceinline__ bool column_sum(const float* __restrict__ part, int slots, int64_t stride, int64_t n, int64_t* col, double* sum)
+{
+    __shared__ double s[64][17];
+    const int c = threadIdx.x & 15, row = threadIdx.x >> 4;
+    *col = (int64_t)blockIdx.x * 16 + c;
+    double a = 0.0;
+    if (*col < n) {
+        const float* q = part + (int64_t)row * stride + *col;
+        int i = row;
+        for (; i + 192 < slots; i += 256, q += 256 * stride) {          // four loads in flight
+            const float v0 = q[0], v1 = q[64 * stride], v2 = q[128 * stride], v3 = q[192 * stride];
+            a += ((double)v0 + v1) + ((double)v2 + v3);
+        }
+        for (; i < slots; i += 64, q += 64 * stride) a += *q;
+    }
+    s[row][c] = a;
+    __syncthreads();
+    if (row < 8) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) a += s[row + 8 * i][c];
+        s[row][c] = a;
+    }
+    __syncthreads();
+    if (row) return false;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a += s[i][c];
+    *sum = a;
+    return *col < n;
 }
