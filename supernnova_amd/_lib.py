@@ -154,15 +154,15 @@ SIGNATURES = {
                                       ctypes.c_int64, _P]),
     "snn_adam_step_clipped": (ctypes.c_int, [ctypes.c_int64, _P, _P, _P, _P, ctypes.c_int64] + [ctypes.c_float] * 6 + [_P, _P]),
     "snn_sgd_step_clipped": (ctypes.c_int, [ctypes.c_int64, _P, _P, _P, ctypes.c_int64] + [ctypes.c_float] * 4 + [_P, _P]),
-    "snn_conv_forward": (ctypes.c_int, [ctypes.POINTER(SnnConvArgs), _P]),
-    "snn_conv_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(SnnConvArgs)]),
-    "snn_conv_backward": (ctypes.c_int, [ctypes.POINTER(SnnConvArgs), _P]),
-    "snn_conv_step": (ctypes.c_int, [ctypes.POINTER(SnnConvArgs), _P]),
-    "snn_scan_tape_floats": (ctypes.c_int64, [ctypes.POINTER(SnnScanArgs)]),
-    "snn_scan_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(SnnScanArgs), ctypes.c_int32]),
-    "snn_scan_forward": (ctypes.c_int, [ctypes.POINTER(SnnScanArgs), _P]),
-    "snn_scan_backward": (ctypes.c_int, [ctypes.POINTER(SnnScanArgs), _P]),
-    "snn_scan_step": (ctypes.c_int, [ctypes.POINTER(SnnScanArgs), _P]),
+    "snn_conv_forward": (ctypes.c_int, [_P, _P]),
+    "snn_conv_workspace_bytes": (ctypes.c_int64, [_P]),
+    "snn_conv_backward": (ctypes.c_int, [_P, _P]),
+    "snn_conv_step": (ctypes.c_int, [_P, _P]),
+    "snn_scan_tape_floats": (ctypes.c_int64, [_P]),
+    "snn_scan_workspace_bytes": (ctypes.c_int64, [_P, ctypes.c_int32]),
+    "snn_scan_forward": (ctypes.c_int, [_P, _P]),
+    "snn_scan_backward": (ctypes.c_int, [_P, _P]),
+    "snn_scan_step": (ctypes.c_int, [_P, _P]),
 }
 
 _lib = None

@@ -4,6 +4,7 @@ batching plan, and launches the kernels on torch's current HIP stream.
 PyTorch is plumbing here (allocator, streams); all arithmetic of the hot path
 runs in libsnn_hip.so.  Nothing in this module computes on the CPU.
 """
+import array
 import contextlib
 import ctypes
 import math
@@ -23,9 +24,12 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on_device(device):
     """Context in which launches go to `device`'s current stream (nothing to do where it is the current device)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _require_cuda(t, name):
@@ -534,45 +538,51 @@ def _dense(t):
 
 def _clip(tensors, max_norm, norm_type, grad_scale, out):
     """One call of snn_clip_grads: device tensor (2,) of the norm and the coefficient min(1, max_norm / (norm + 1e-6))."""
-    src = list(tensors)
-    try:
-        code = _NORM_TYPES[float(norm_type)]
-    except KeyError:
-        raise L.SnnError(f"norm_type {norm_type!r}: supported are 1, 2 and inf") from None
+    src = tensors if type(tensors) is list else list(tensors)
+    code = _NORM_TYPES.get(norm_type)
+    if code is None:
+        raise L.SnnError(f"norm_type {norm_type!r}: supported are 1, 2 and inf")
     if not src:
         raise L.SnnError("no gradients")
     dev = src[0].device
     if dev.type != "cuda":
         raise L.SnnError("gradients must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")
+    # whole-list passes: a model has hundreds of gradients, and a line of Python for each costs more than its share of the kernel
     try:
         dts = [_DTYPES[t.dtype] for t in src]
     except KeyError as e:
         raise L.SnnError(f"gradients of type {e.args[0]}: supported are float32, bfloat16 and float16") from None
-    for t in src:
-        if t.device != dev or not (t.is_contiguous() or _dense(t)):
-            raise L.SnnError("gradients must be dense tensors (no gaps, no repeated elements) on one device")
+    whole = all([t.is_contiguous() for t in src])
+    if [t.get_device() for t in src].count(dev.index) != len(src) or not (whole or all(_dense(t) for t in src)):
+        raise L.SnnError("gradients must be dense tensors (no gaps, no repeated elements) on one device")
     n = len(src)
-    ptrs = [t.data_ptr() for t in src]
+    numel = array.array("q", [t.numel() for t in src])
+    ptrs = array.array("Q", [t.data_ptr() for t in src])
     dst = None
     if out is not None:
-        out = list(out)
-        full = [p for p, t in zip(ptrs, src) if t.numel()]
-        if len(set(full)) != len(full):
-            raise L.SnnError("a gradient is listed twice")
-        if len(out) != n:
-            raise L.SnnError(f"out has {len(out)} tensors for {n} gradients")
-        for t, o in zip(src, out):
-            if o is not t and (o.shape != t.shape or o.dtype != t.dtype or o.device != dev or
-                               (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()))):
+        if len(set(ptrs)) != n:
+            full = [p for p, k in zip(ptrs, numel) if k]
+            if len(set(full)) != len(full):
+                raise L.SnnError("a gradient is listed twice")
+        if out is src:
+            dst = ptrs
+        else:
+            out = list(out)
+            if len(out) != n:
+                raise L.SnnError(f"out has {len(out)} tensors for {n} gradients")
+            if [o.shape for o in out] != [t.shape for t in src] or [o.dtype for o in out] != [t.dtype for t in src] or \
+                    [o.get_device() for o in out].count(dev.index) != n or \
+                    not (whole and all([o.is_contiguous() for o in out]) or [o.stride() for o in out] == [t.stride() for t in src]):
                 raise L.SnnError("out must match the gradients in shape, strides, type and device")
-        dst = (ctypes.c_void_p * n)(*[o.data_ptr() for o in out])
+            dst = array.array("Q", [o.data_ptr() for o in out])
     lib = L.load()
-    numel = (ctypes.c_int64 * n)(*[t.numel() for t in src])
-    doubles = L.check(lib.snn_clip_scratch_doubles(n, numel), "snn_clip_scratch_doubles")
+    dts = array.array("i", dts)
+    at = numel.buffer_info()[0]
+    doubles = L.check(lib.snn_clip_scratch_doubles(n, at), "snn_clip_scratch_doubles")
+    buf = torch.empty(1 + doubles, dtype=torch.float64, device=dev)
+    p = buf.data_ptr()
     with _on_device(dev):
-        buf = torch.empty(1 + doubles, dtype=torch.float64, device=dev)
-        p = buf.data_ptr()
-        L.check(lib.snn_clip_grads(n, (ctypes.c_void_p * n)(*ptrs), dst, numel, (ctypes.c_int32 * n)(*dts),
+        L.check(lib.snn_clip_grads(n, ptrs.buffer_info()[0], None if dst is None else dst.buffer_info()[0], at, dts.buffer_info()[0],
                                    code, max_norm, grad_scale, p, p + 8, doubles, _stream()), "snn_clip_grads")
     return buf[:1].view(torch.float32)
 

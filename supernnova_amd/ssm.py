@@ -25,6 +25,8 @@ a backward pass while a stream is being captured (autograd would accumulate on t
 in before): capture the explicit pair.  The step functions write the state in place unless given `new_state`.
 """
 import ctypes
+import functools
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -33,7 +35,12 @@ from torch.autograd.function import once_differentiable
 from . import _lib as L
 from . import engine as E
 
-_NONE = L.SnnView(None, 0, 0)
+# snn_conv_args / snn_scan_args, packed field by field: a tenth of the time ctypes takes to fill its structures, which at one
+# token a call is as long as the kernel runs
+_CONV = struct.Struct("@iiqPP4i" + 4 * "Pqq" + "9Pq")
+_SCAN = struct.Struct("@iiqPP6i" + 6 * "Pqq" + "2q6Pq" + 6 * "Pqq" + "6Pq")
+assert _CONV.size == ctypes.sizeof(L.SnnConvArgs) and _SCAN.size == ctypes.sizeof(L.SnnScanArgs)
+_NO_VIEW = (0, 0, 0)
 
 
 class ConvGrads(NamedTuple):
@@ -59,83 +66,97 @@ def _fail(msg):
     raise L.SnnError(msg)
 
 
-def _param(t, name, shape, device):
-    """A contiguous float32 parameter or state -> its address (None stays None)."""
-    if t is None:
-        return None
-    E._require_cuda(t, name)
-    if t.shape != shape or t.device != device:
-        _fail(f"{name} must be {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+def _on_gpu(x):
+    if not x.is_cuda:
+        _fail("x must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")
 
 
 class _Batch:
     """The layout of one call: sequences, steps, and the strides of a tensor's step and sequence dimensions."""
 
     def __init__(self, x, lengths, offsets, max_len, time_major):
-        if not x.is_cuda:
-            _fail("x must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")
+        _on_gpu(x)
         if x.dtype not in E._DTYPES:
             _fail(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-        self.dtype, self.device, self.D = x.dtype, x.device, x.size(-1) if x.dim() else 0
+        shape = x.shape
+        self.dtype, self.device, self.index, self.shape = x.dtype, x.device, x.get_device(), shape
+        lengths_p = offsets_p = rows = 0
         if offsets is not None:
-            if x.dim() != 2:
-                _fail(f"ragged rows must be (rows, channels), got {tuple(x.shape)}")
+            if len(shape) != 2:
+                _fail(f"ragged rows must be (rows, channels), got {tuple(shape)}")
             if lengths is not None:
                 _fail("lengths and offsets exclude each other")
-            self._index(offsets, "offsets", torch.int64, None)
-            self.B, rows = offsets.numel() - 1, x.size(0)
+            offsets_p = self._vector(offsets, "offsets", torch.int64, None)
+            self.B, rows = offsets.numel() - 1, shape[0]
             self.T = rows if max_len is None else min(int(max_len), rows)
-            self.t_dim, self.n_dim, lead = 0, None, 1
+            self.t_dim, self.n_dim, self.lead = 0, None, shape[:1]
         else:
-            if x.dim() != 3:
-                _fail(f"x must be 3-D (or 2-D rows with offsets), got {tuple(x.shape)}")
+            if len(shape) != 3:
+                _fail(f"x must be 3-D (or 2-D rows with offsets), got {tuple(shape)}")
             if max_len is not None:
                 _fail("max_len goes with offsets")
             self.t_dim, self.n_dim = (0, 1) if time_major else (1, 0)
-            self.T, self.B, rows, lead = x.size(self.t_dim), x.size(self.n_dim), 0, 2
+            self.T, self.B, self.lead = shape[self.t_dim], shape[self.n_dim], shape[:2]
             if lengths is not None:
-                self._index(lengths, "lengths", torch.int32, self.B)
-        self.lead = x.shape[:lead]
+                lengths_p = self._vector(lengths, "lengths", torch.int32, self.B)
+        self.D = shape[-1]
         if self.T < 1 or self.B < 1 or self.D < 1:
-            _fail(f"need at least one sequence, one step and one channel, got x {tuple(x.shape)}, {self.B} sequences, {self.T} steps")
+            _fail(f"need at least one sequence, one step and one channel, got x {tuple(shape)}, {self.B} sequences, {self.T} steps")
         if max(self.T, self.B, self.D) >= 1 << 31:
             _fail("sizes must fit 31 bits")
-        self.seq = L.SnnSeq(self.B, self.T, rows, None if lengths is None else lengths.data_ptr(),
-                            None if offsets is None else offsets.data_ptr())
+        self.seq = (self.B, self.T, rows, lengths_p, offsets_p)
 
-    def _index(self, t, name, dtype, n):
-        if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or t.device != self.device or t.numel() < 1 or (n is not None and t.numel() != n):
+    def _vector(self, t, name, dtype, n):
+        if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or t.get_device() != self.index or t.numel() < 1 or (n is not None and t.numel() != n):
             _fail(f"{name} must be a contiguous {dtype} vector{'' if n is None else f' of {n}'} on {self.device}")
+        return t.data_ptr()
 
     def view(self, t, name, shape=None):
         """A tensor of the batch (default: of x's shape) as snn_view."""
-        if t.dtype != self.dtype or t.device != self.device or t.shape != (self.lead + (self.D,) if shape is None else shape):
-            _fail(f"{name} must be {self.dtype} {tuple(self.lead + (self.D,) if shape is None else shape)} on {self.device}, "
+        if t.dtype != self.dtype or t.get_device() != self.index or t.shape != (self.shape if shape is None else shape):
+            _fail(f"{name} must be {self.dtype} {tuple(self.shape if shape is None else shape)} on {self.device}, "
                   f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if t.stride(-1) != 1 and t.size(-1) != 1:
+        st = t.stride()
+        if st[-1] != 1 and t.size(-1) != 1:
             _fail(f"{name}: the last dimension must have unit stride")
-        return L.SnnView(t.data_ptr(), t.stride(self.t_dim), 0 if self.n_dim is None else t.stride(self.n_dim))
+        return t.data_ptr(), st[self.t_dim], 0 if self.n_dim is None else st[self.n_dim]
 
-    def out(self, t):
-        return L.SnnView(t.data_ptr(), t.stride(self.t_dim), 0 if self.n_dim is None else t.stride(self.n_dim))
+    def empty(self, shape=None):
+        """A contiguous result of x's (or the given) shape, and its snn_view."""
+        t = torch.empty(self.shape if shape is None else shape, dtype=self.dtype, device=self.device)
+        st = t.stride()
+        return t, (t.data_ptr(), st[self.t_dim], 0 if self.n_dim is None else st[self.n_dim])
 
-    def empty(self, *tail):
-        return torch.empty(self.lead + (tail or (self.D,)), dtype=self.dtype, device=self.device)
+    def param(self, t, name, shape, dtype=torch.float32):
+        """A contiguous parameter or state -> its address (None: 0)."""
+        if t is None:
+            return 0
+        if t.dtype != dtype or t.get_device() != self.index or t.shape != shape or not t.is_contiguous():
+            _fail(f"{name} must be contiguous {dtype} {shape} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t.data_ptr()
+
+    def floats(self, *shape):
+        return torch.empty(shape, dtype=torch.float32, device=self.device)
+
+    def launch(self, fn, what, args):
+        if self.index == torch.cuda.current_device():
+            L.check(fn(args, torch._C._cuda_getCurrentRawStream(self.index)), what)
+        else:
+            with torch.cuda.device(self.index):
+                L.check(fn(args, torch._C._cuda_getCurrentRawStream(self.index)), what)
 
 
 class _Step(_Batch):
     """One step of B sequences: x (B, D)."""
 
     def __init__(self, x):
-        if not x.is_cuda:
-            _fail("x must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")
+        _on_gpu(x)
         if x.dtype not in E._DTYPES or x.dim() != 2 or x.numel() < 1:
             _fail(f"x must be a non-empty (sequences, channels) tensor of float32, bfloat16 or float16, got {x.dtype} {tuple(x.shape)}")
-        self.dtype, self.device = x.dtype, x.device
-        self.B, self.D = x.shape
-        self.T, self.t_dim, self.n_dim, self.lead = 1, 0, 0, x.shape[:1]
-        self.seq = L.SnnSeq(self.B, 1, 0, None, None)
+        self.dtype, self.device, self.index, self.shape = x.dtype, x.device, x.get_device(), x.shape
+        self.B, self.D = self.shape
+        self.T, self.t_dim, self.n_dim, self.lead = 1, 0, 0, self.shape[:1]
+        self.seq = (self.B, 1, 0, 0, 0)
 
 
 def _unit(t):
@@ -144,31 +165,14 @@ def _unit(t):
 
 
 # ------------------------------------------------------------------------------------------------- convolution
-def _conv_args(bt, x, weight, bias, activation, state, state_name="initial_state"):
+def _conv_head(bt, weight, bias, activation):
     if activation not in ("silu", None):
         _fail(f"activation must be 'silu' or None, got {activation!r}")
     if weight.dim() != 2 or not 2 <= weight.size(1) <= 4:
         _fail(f"weight must be (channels, 2..4), got {tuple(weight.shape)}")
     W = weight.size(1)
-    a = L.SnnConvArgs(seq=bt.seq, dtype=E._DTYPES[bt.dtype], channels=bt.D, width=W, silu=activation == "silu")
-    a.x = bt.view(x, "x")
-    a.weight = _param(weight, "weight", (bt.D, W), bt.device)
-    a.bias = _param(bias, "bias", (bt.D,), bt.device)
-    a.state_in = _conv_state(bt, state, state_name, W)
-    return a, W
-
-
-def _conv_state(bt, t, name, W):
-    if t is None:
-        return None
-    if t.dtype != bt.dtype or t.shape != (bt.B, W - 1, bt.D) or t.device != bt.device or not t.is_contiguous():
-        _fail(f"{name} must be contiguous {bt.dtype} {(bt.B, W - 1, bt.D)} on {bt.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
-
-
-def _launch(fn, what, a, device):
-    with E._on_device(device):
-        L.check(fn(ctypes.byref(a), E._stream()), what)
+    return W, (*bt.seq, E._DTYPES[bt.dtype], bt.D, W, activation == "silu"), \
+        (bt.param(weight, "weight", (bt.D, W)), bt.param(bias, "bias", (bt.D,)))
 
 
 def causal_conv_forward(x, weight, bias=None, *, activation="silu", lengths=None, offsets=None, max_len=None,
@@ -177,14 +181,12 @@ def causal_conv_forward(x, weight, bias=None, *, activation="silu", lengths=None
     None, activation "silu" or None.  Returns (y like x, final state (B, W - 1, D) or None); the final state is what
     causal_conv_step and a later call's initial_state go on from."""
     bt = _Batch(x, lengths, offsets, max_len, time_major)
-    a, W = _conv_args(bt, x, weight, bias, activation, initial_state)
-    y = bt.empty()
-    a.y = bt.out(y)
-    end = None
-    if want_final_state:
-        end = torch.empty((bt.B, W - 1, bt.D), dtype=bt.dtype, device=bt.device)
-        a.state_out = end.data_ptr()
-    _launch(L.load().snn_conv_forward, "snn_conv_forward", a, bt.device)
+    W, head, par = _conv_head(bt, weight, bias, activation)
+    vx, state = bt.view(x, "x"), bt.param(initial_state, "initial_state", (bt.B, W - 1, bt.D), bt.dtype)
+    y, vy = bt.empty()
+    end = torch.empty((bt.B, W - 1, bt.D), dtype=bt.dtype, device=bt.device) if want_final_state else None
+    bt.launch(L.load().snn_conv_forward, "snn_conv_forward",
+              _CONV.pack(*head, *vx, *vy, *_NO_VIEW, *_NO_VIEW, *par, state, 0 if end is None else end.data_ptr(), 0, 0, 0, 0, 0, 0))
     return y, end
 
 
@@ -193,25 +195,20 @@ def causal_conv_backward(x, weight, bias, dy, *, dfinal_state=None, activation="
     """Gradients of causal_conv_forward's result from dy = dloss/dy and, if the final state was used, dfinal_state.  Sums over
     sequences and steps are taken in an order that depends on the sizes alone."""
     bt = _Batch(x, lengths, offsets, max_len, time_major)
-    a, W = _conv_args(bt, x, weight, bias, activation, initial_state)
-    dy = _unit(dy)
-    a.dy = bt.view(dy, "dy")
-    a.dstate_out = _conv_state(bt, dfinal_state, "dfinal_state", W)
-    dx = bt.empty()
-    a.dx = bt.out(dx)
-    dpar = torch.empty(bt.D * (W + 1), dtype=torch.float32, device=bt.device)
-    a.dweight = dpar.data_ptr()
-    if bias is not None:
-        a.dbias = a.dweight + 4 * bt.D * W
-    dstate = None
-    if initial_state is not None:
-        dstate = torch.empty_like(initial_state)
-        a.dstate_in = dstate.data_ptr()
+    W, head, par = _conv_head(bt, weight, bias, activation)
+    dy, shape = _unit(dy), (bt.B, W - 1, bt.D)
+    vx, vdy, state = bt.view(x, "x"), bt.view(dy, "dy"), bt.param(initial_state, "initial_state", shape, bt.dtype)
+    dend = bt.param(dfinal_state, "dfinal_state", shape, bt.dtype)
+    dx, vdx = bt.empty()
+    dweight, dbias = bt.floats(bt.D, W), bt.floats(bt.D) if bias is not None else None
+    dstate = torch.empty_like(initial_state) if initial_state is not None else None
+    args = (*head, *vx, *_NO_VIEW, *vdy, *vdx, *par, state, 0, dend, 0 if dstate is None else dstate.data_ptr(), dweight.data_ptr(),
+            0 if dbias is None else dbias.data_ptr())
     lib = L.load()
-    ws = torch.empty(L.check(lib.snn_conv_workspace_bytes(ctypes.byref(a)), "snn_conv_workspace_bytes"), dtype=torch.uint8, device=bt.device)
-    a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
-    _launch(lib.snn_conv_backward, "snn_conv_backward", a, bt.device)
-    return ConvGrads(dx, dpar[:bt.D * W].view(bt.D, W), dpar[bt.D * W:] if bias is not None else None, dstate)
+    need = L.check(lib.snn_conv_workspace_bytes(_CONV.pack(*args, 0, 0)), "snn_conv_workspace_bytes")
+    ws = bt.floats(need // 4)
+    bt.launch(lib.snn_conv_backward, "snn_conv_backward", _CONV.pack(*args, ws.data_ptr(), need))
+    return ConvGrads(dx, dweight, dbias, dstate)
 
 
 def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_state=None):
@@ -220,57 +217,60 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_stat
     bt = _Step(x)
     if state is None:
         _fail("causal_conv_step needs the state")
-    a, W = _conv_args(bt, x, weight, bias, activation, state, "state")
-    a.state_out = a.state_in if new_state is None else _conv_state(bt, new_state, "new_state", W)
-    y = bt.empty()
-    a.y = bt.out(y)
-    _launch(L.load().snn_conv_step, "snn_conv_step", a, bt.device)
+    W, head, par = _conv_head(bt, weight, bias, activation)
+    shape = (bt.B, W - 1, bt.D)
+    vx, old = bt.view(x, "x"), bt.param(state, "state", shape, bt.dtype)
+    new = old if new_state is None else bt.param(new_state, "new_state", shape, bt.dtype)
+    y, vy = bt.empty()
+    bt.launch(L.load().snn_conv_step, "snn_conv_step", _CONV.pack(*head, *vx, *vy, *_NO_VIEW, *_NO_VIEW, *par, old, new, 0, 0, 0, 0, 0, 0))
     return y
 
 
 # ------------------------------------------------------------------------------------------------- scan
-def _scan_args(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, state, state_name="initial_state"):
+@functools.lru_cache(maxsize=256)
+def _scan_sizes(dtype, D, N, G, B, T, rows, ragged):
+    """(tape floats, forward workspace bytes, backward workspace bytes): they depend on the sizes alone."""
+    a = L.SnnScanArgs(seq=L.SnnSeq(B, T, rows, None, 8 if ragged else None), dtype=dtype, channels=D, states=N, groups=G)
+    lib, p = L.load(), ctypes.byref(a)
+    return (L.check(lib.snn_scan_tape_floats(p), "snn_scan_tape_floats"), L.check(lib.snn_scan_workspace_bytes(p, 0), "snn_scan_workspace_bytes"),
+            L.check(lib.snn_scan_workspace_bytes(p, 1), "snn_scan_workspace_bytes"))
+
+
+def _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, y):
+    """The fields up to delta_bias (y: its view), and G, N, the shape of B and C, and the sizes."""
     if A.dim() != 2 or not 1 <= A.size(1) <= 64:
         _fail(f"A must be (channels, 1..64), got {tuple(A.shape)}")
-    N, lead = A.size(1), len(bt.lead)
-    if B.dim() not in (lead + 1, lead + 2) or B.shape != C.shape:
+    N, lead, dims = A.size(1), len(bt.lead), B.dim()
+    if dims not in (lead + 1, lead + 2) or B.shape != C.shape:
         _fail(f"B and C must be alike, (.., states) or (.., groups, states), got {tuple(B.shape)} and {tuple(C.shape)}")
-    G = B.size(-2) if B.dim() == lead + 2 else 1
+    G = B.size(-2) if dims == lead + 2 else 1
     if G < 1 or bt.D % G:
         _fail(f"{bt.D} channels cannot be dealt to {G} groups")
-    shape = bt.lead + ((G, N) if B.dim() == lead + 2 else (N,))
-    a = L.SnnScanArgs(seq=bt.seq, dtype=E._DTYPES[bt.dtype], channels=bt.D, states=N, groups=G, softplus=bool(delta_softplus))
-    a.x, a.delta = bt.view(x, "x"), bt.view(delta, "delta")
-    a.z = _NONE if z is None else bt.view(z, "z")
-    a.B, a.C = bt.view(B, "B", shape), bt.view(C, "C", shape)
-    if G > 1:
-        a.B_stride_g, a.C_stride_g = B.stride(-2), C.stride(-2)
-    a.A = _param(A, "A", (bt.D, N), bt.device)
-    a.skip = _param(D, "D", (bt.D,), bt.device)
-    a.delta_bias = _param(delta_bias, "delta_bias", (bt.D,), bt.device)
-    a.state_in = _param(state, state_name, (bt.B, bt.D, N), bt.device)
-    return a, G, N
+    shape = bt.lead + ((G, N) if dims == lead + 2 else (N,))
+    dt = E._DTYPES[bt.dtype]
+    head = (*bt.seq, dt, bt.D, N, G, bool(delta_softplus), 0, *bt.view(x, "x"), *bt.view(delta, "delta"),
+            *(_NO_VIEW if z is None else bt.view(z, "z")), *bt.view(B, "B", shape), *bt.view(C, "C", shape), *y,
+            B.stride(-2) if G > 1 else 0, C.stride(-2) if G > 1 else 0,
+            bt.param(A, "A", (bt.D, N)), bt.param(D, "D", (bt.D,)), bt.param(delta_bias, "delta_bias", (bt.D,)))
+    return head, G, N, shape
+
+
+_NO_GRADS = (*(6 * _NO_VIEW), 0, 0, 0, 0, 0)
 
 
 def _scan_forward(x, delta, A, B, C, D, z, delta_bias, delta_softplus, lengths, offsets, max_len, initial_state, want_final_state,
                   time_major, want_tape):
     bt = _Batch(x, lengths, offsets, max_len, time_major)
-    a, _, N = _scan_args(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, initial_state)
-    y = bt.empty()
-    a.y = bt.out(y)
-    end = tape = None
-    if want_final_state:
-        end = torch.empty((bt.B, bt.D, N), dtype=torch.float32, device=bt.device)
-        a.state_out = end.data_ptr()
-    lib = L.load()
-    if want_tape:
-        tape = torch.empty(L.check(lib.snn_scan_tape_floats(ctypes.byref(a)), "snn_scan_tape_floats"), dtype=torch.float32, device=bt.device)
-        a.tape, a.tape_floats = tape.data_ptr(), tape.numel()
-    need = L.check(lib.snn_scan_workspace_bytes(ctypes.byref(a), 0), "snn_scan_workspace_bytes")
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=bt.device)
-        a.ws, a.ws_bytes = ws.data_ptr(), need
-    _launch(lib.snn_scan_forward, "snn_scan_forward", a, bt.device)
+    y, vy = bt.empty()
+    head, G, N, _ = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, vy)
+    state = bt.param(initial_state, "initial_state", (bt.B, bt.D, N))
+    n_tape, need, _ = _scan_sizes(head[5], bt.D, N, G, bt.B, bt.T, bt.seq[2], offsets is not None)
+    end = bt.floats(bt.B, bt.D, N) if want_final_state else None
+    tape = bt.floats(n_tape) if want_tape else None
+    ws = bt.floats(need // 4) if need else None
+    bt.launch(L.load().snn_scan_forward, "snn_scan_forward",
+              _SCAN.pack(*head, state, 0 if end is None else end.data_ptr(), 0 if tape is None else tape.data_ptr(), n_tape if want_tape else 0,
+                         *_NO_GRADS, 0 if ws is None else ws.data_ptr(), need))
     return y, end, tape
 
 
@@ -295,37 +295,23 @@ def selective_scan_backward(x, delta, A, B, C, dy, tape, D=None, z=None, delta_b
     """Gradients from dy = dloss/dy and, if the final state was used, dfinal_state, with the tape of selective_scan_train over the
     same inputs.  Every sum is taken in an order that depends on the sizes alone."""
     bt = _Batch(x, lengths, offsets, max_len, time_major)
-    a, G, N = _scan_args(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, initial_state)
-    dev, Dm = bt.device, bt.D
-    dy = _unit(dy)
-    a.dy = bt.view(dy, "dy")
-    a.dstate_out = _param(dfinal_state, "dfinal_state", (bt.B, Dm, N), dev)
-    E._require_cuda(tape, "tape")
-    a.tape, a.tape_floats = tape.data_ptr(), tape.numel()
-    dx, ddelta = bt.empty(), bt.empty()
-    a.dx, a.ddelta = bt.out(dx), bt.out(ddelta)
-    dz = None
-    if z is not None:
-        dz = bt.empty()
-        a.dz = bt.out(dz)
-    dB, dC = bt.empty(*B.shape[len(bt.lead):]), bt.empty(*C.shape[len(bt.lead):])
-    a.dB, a.dC = bt.out(dB), bt.out(dC)
-    dpar = torch.empty(Dm * (N + 2), dtype=torch.float32, device=dev)
-    a.dA = dpar.data_ptr()
-    if D is not None:
-        a.dskip = a.dA + 4 * Dm * N
-    if delta_bias is not None:
-        a.ddelta_bias = a.dA + 4 * Dm * (N + 1)
-    dstate = None
-    if initial_state is not None:
-        dstate = torch.empty_like(initial_state)
-        a.dstate_in = dstate.data_ptr()
-    lib = L.load()
-    ws = torch.empty(L.check(lib.snn_scan_workspace_bytes(ctypes.byref(a), 1), "snn_scan_workspace_bytes"), dtype=torch.uint8, device=dev)
-    a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
-    _launch(lib.snn_scan_backward, "snn_scan_backward", a, dev)
-    return ScanGrads(dx, ddelta, dpar[:Dm * N].view(Dm, N), dB, dC, dpar[Dm * N:Dm * (N + 1)] if D is not None else None, dz,
-                     dpar[Dm * (N + 1):] if delta_bias is not None else None, dstate)
+    head, G, N, shape = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, _NO_VIEW)
+    dy, Dm, sizes = _unit(dy), bt.D, (bt.B, bt.D, N)
+    vdy, state, dend = bt.view(dy, "dy"), bt.param(initial_state, "initial_state", sizes), bt.param(dfinal_state, "dfinal_state", sizes)
+    n_tape, _, need = _scan_sizes(head[5], Dm, N, G, bt.B, bt.T, bt.seq[2], offsets is not None)
+    if tape.numel() < n_tape:
+        _fail(f"the tape is too small: {tape.numel()} floats, {n_tape} needed (of selective_scan_train over the same inputs)")
+    tape_p = bt.param(tape, "tape", tape.shape)
+    (dx, vdx), (ddelta, vdd), (dB, vdB), (dC, vdC) = bt.empty(), bt.empty(), bt.empty(shape), bt.empty(shape)
+    dz, vdz = bt.empty() if z is not None else (None, _NO_VIEW)
+    dA, dD = bt.floats(Dm, N), bt.floats(Dm) if D is not None else None
+    dbias = bt.floats(Dm) if delta_bias is not None else None
+    dstate = torch.empty_like(initial_state) if initial_state is not None else None
+    ws = bt.floats(need // 4)
+    bt.launch(L.load().snn_scan_backward, "snn_scan_backward",
+              _SCAN.pack(*head, state, 0, tape_p, n_tape, *vdy, *vdx, *vdd, *vdz, *vdB, *vdC, dend, dA.data_ptr(), 0 if dD is None else dD.data_ptr(),
+                         0 if dbias is None else dbias.data_ptr(), 0 if dstate is None else dstate.data_ptr(), ws.data_ptr(), need))
+    return ScanGrads(dx, ddelta, dA, dB, dC, dD, dz, dbias, dstate)
 
 
 def selective_scan_step(x, state, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_softplus=True, new_state=None):
@@ -334,11 +320,11 @@ def selective_scan_step(x, state, delta, A, B, C, D=None, z=None, delta_bias=Non
     bt = _Step(x)
     if state is None:
         _fail("selective_scan_step needs the state")
-    a, _, N = _scan_args(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, state, "state")
-    a.state_out = a.state_in if new_state is None else _param(new_state, "new_state", (bt.B, bt.D, N), bt.device)
-    y = bt.empty()
-    a.y = bt.out(y)
-    _launch(L.load().snn_scan_step, "snn_scan_step", a, bt.device)
+    y, vy = bt.empty()
+    head, _, N, _ = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, vy)
+    old = bt.param(state, "state", (bt.B, bt.D, N))
+    new = old if new_state is None else bt.param(new_state, "new_state", (bt.B, bt.D, N))
+    bt.launch(L.load().snn_scan_step, "snn_scan_step", _SCAN.pack(*head, old, new, 0, 0, *_NO_GRADS, 0, 0))
     return y
 
 
