@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr int CLIP_TENSORS = 96, CLIP_PIECE = 1 << 15, CLIP_DIRECT = 1024;
+constexpr int CLIP_TENSORS = 96, CLIP_PIECE = 1 << 14, CLIP_DIRECT = 1024;
 
 struct Table {                                  // 2.7 KB of the 4 KB of kernel arguments
     const void* src[CLIP_TENSORS];
@@ -206,14 +206,17 @@ __global__ void __launch_bounds__(256) sgd_clipped_kernel(int64_t n, float* __re
 
 int64_t pieces_of(int64_t n) { return (n + CLIP_PIECE - 1) / CLIP_PIECE; }
 
-// tables of up to CLIP_TENSORS non-empty tensors, one launch of `f(table, pieces of the table, pieces before it)` each
-template <typename F> void each_table(int n_tensors, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, F f)
+// tables of up to CLIP_TENSORS non-empty tensors, one launch of `f(table, pieces of the table, pieces before it)` each; `back`:
+// from the last tensor to the first
+template <typename F>
+void each_table(int n_tensors, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, bool back, F f)
 {
     Table t;
     t.count = 0;
     int64_t before = 0;
     int here = 0;
-    for (int i = 0; i < n_tensors; ++i) {
+    for (int k = 0; k < n_tensors; ++k) {
+        const int i = back ? n_tensors - 1 - k : k;
         if (numel[i]) {
             t.src[t.count] = src[i];
             t.dst[t.count] = dst ? dst[i] : nullptr;
@@ -223,7 +226,7 @@ template <typename F> void each_table(int n_tensors, const void* const* src, voi
             here += (int)pieces_of(numel[i]);
             t.first[++t.count] = here;
         }
-        if (t.count && (t.count == CLIP_TENSORS || i == n_tensors - 1)) {
+        if (t.count && (t.count == CLIP_TENSORS || k == n_tensors - 1)) {
             f(t, here, before);
             before += here;
             here = t.count = 0;
@@ -236,13 +239,13 @@ void run(int n_tensors, const void* const* src, void* const* dst, const int64_t*
          float* out, double* part, int64_t pieces, hipStream_t s)
 {
     const dim3 w(256);
-    each_table(n_tensors, src, dst, numel, dtype, [&](const Table& t, int here, int64_t before) {
+    each_table(n_tensors, src, dst, numel, dtype, false, [&](const Table& t, int here, int64_t before) {
         hipLaunchKernelGGL((clip_norm_kernel<P>), dim3(here), w, 0, s, t, part + before);
     });
     const bool direct = dst && pieces && pieces <= CLIP_DIRECT;
     if (!direct) hipLaunchKernelGGL((clip_finish_kernel<P>), dim3(1), dim3(1024), 0, s, (const double*)part, (int)pieces, max_norm, grad_scale, out);
-    if (dst)
-        each_table(n_tensors, src, dst, numel, dtype, [&](const Table& t, int here, int64_t before) {
+    if (dst)            // backwards: what the first pass read last is still in the last-level cache
+        each_table(n_tensors, src, dst, numel, dtype, true, [&](const Table& t, int here, int64_t before) {
             if (direct)
                 hipLaunchKernelGGL((clip_scale_kernel<P, true>), dim3(here), w, 0, s, t, (const double*)part, (int)pieces, max_norm, grad_scale, out, before == 0);
             else

@@ -575,6 +575,10 @@ def _clip(tensors, max_norm, norm_type, grad_scale, out):
                     not (whole and all([o.is_contiguous() for o in out]) or [o.stride() for o in out] == [t.stride() for t in src]):
                 raise L.SnnError("out must match the gradients in shape, strides, type and device")
             dst = array.array("Q", [o.data_ptr() for o in out])
+            full = [(d, s) for d, s, k in zip(dst, ptrs, numel) if k]
+            apart = {d for d, s in full}
+            if len(apart) != len(full) or any(s in apart and s != d for d, s in full):
+                raise L.SnnError("out lists a tensor twice, or the place of another gradient")
     lib = L.load()
     dts = array.array("i", dts)
     at = numel.buffer_info()[0]

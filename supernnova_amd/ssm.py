@@ -159,6 +159,14 @@ class _Step(_Batch):
         self.seq = (self.B, 1, 0, 0, 0)
 
 
+def _apart(state, new_state, address):
+    """new_state's address; the two may be one buffer, but must not overlap in part (other sequences would read what is written)."""
+    gap = abs(address - state.data_ptr())
+    if 0 < gap < state.numel() * state.element_size():
+        _fail("state and new_state overlap")
+    return address
+
+
 def _unit(t):
     """Gradients arrive with whatever strides autograd chose (an expanded sum has none): rows of unit stride."""
     return t if t.stride(-1) == 1 else t.contiguous()
@@ -220,7 +228,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_stat
     W, head, par = _conv_head(bt, weight, bias, activation)
     shape = (bt.B, W - 1, bt.D)
     vx, old = bt.view(x, "x"), bt.param(state, "state", shape, bt.dtype)
-    new = old if new_state is None else bt.param(new_state, "new_state", shape, bt.dtype)
+    new = old if new_state is None else _apart(state, new_state, bt.param(new_state, "new_state", shape, bt.dtype))
     y, vy = bt.empty()
     bt.launch(L.load().snn_conv_step, "snn_conv_step", _CONV.pack(*head, *vx, *vy, *_NO_VIEW, *_NO_VIEW, *par, old, new, 0, 0, 0, 0, 0, 0))
     return y
@@ -323,7 +331,7 @@ def selective_scan_step(x, state, delta, A, B, C, D=None, z=None, delta_bias=Non
     y, vy = bt.empty()
     head, _, N, _ = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, vy)
     old = bt.param(state, "state", (bt.B, bt.D, N))
-    new = old if new_state is None else bt.param(new_state, "new_state", (bt.B, bt.D, N))
+    new = old if new_state is None else _apart(state, new_state, bt.param(new_state, "new_state", (bt.B, bt.D, N)))
     bt.launch(L.load().snn_scan_step, "snn_scan_step", _SCAN.pack(*head, old, new, 0, 0, *_NO_GRADS, 0, 0))
     return y
 

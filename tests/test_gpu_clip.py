@@ -108,6 +108,13 @@ def test_dense_orders_and_refusals():
         E.clip_grads([t], 1.0, out=[])
     with pytest.raises(L.SnnError, match="twice"):
         E.clip_grads([t, t], 1.0)
+    u = t.clone()
+    with pytest.raises(L.SnnError, match="another gradient"):
+        E.clip_grads([t, u], 1.0, out=[u, t])
+    with pytest.raises(L.SnnError, match="twice"):
+        E.clip_grads([t, u], 1.0, out=[t, t])
+    with pytest.raises(L.SnnError, match="norm_type"):
+        E.clip_grads([t], 1.0, norm_type="inf")
 
 
 def test_clip_grad_norm_like_torch():

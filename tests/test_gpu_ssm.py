@@ -499,8 +499,59 @@ def test_conv_and_step_refusals():
         ssm.causal_conv_step(x[0], None, w)
     with pytest.raises(L.SnnError, match="new_state"):
         ssm.causal_conv_step(x[0], torch.zeros(2, 3, 8, device="cuda"), w, new_state=torch.zeros(2, 3, 8, device="cuda").half())
+    pool = torch.zeros(3, 3, 8, device="cuda")
+    with pytest.raises(L.SnnError, match="overlap"):
+        ssm.causal_conv_step(x[0], pool[:2], w, new_state=pool[1:])
     with pytest.raises(L.SnnError, match="channels"):
         ssm.causal_conv_step(x, torch.zeros(2, 3, 8, device="cuda"), w)
     y, _, tape = ssm.selective_scan_train(x, x, -torch.ones(8, 4, device="cuda"), x[..., :4], x[..., :4])
     with pytest.raises(L.SnnError, match="too small"):
         ssm.selective_scan_backward(x, x, -torch.ones(8, 4, device="cuda"), x[..., :4], x[..., :4], y, tape[:8])
+
+
+def test_one_state_pool_shifted_by_whole_states_is_allowed():
+    """Disjoint slices of one pool as state and new_state."""
+    pool, x, w = torch.randn(4, 3, 8, device="cuda"), torch.randn(2, 8, device="cuda"), torch.randn(8, 4, device="cuda")
+    want = pool[:2].clone()
+    y = ssm.causal_conv_step(x, want, w)
+    assert torch.equal(ssm.causal_conv_step(x, pool[:2], w, new_state=pool[2:]), y) and torch.equal(pool[2:], want)
+
+
+def test_channels_first_and_odd_strides_through_autograd():
+    """The gradient of a sum has no strides of its own, a transposed result's gradient arrives transposed."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(2, 9, 6, generator=g).cuda().requires_grad_()
+    w = torch.randn(6, 3, generator=g).cuda().requires_grad_()
+    ssm.causal_conv(x, w, time_major=False).sum().backward()
+    a = x.grad.clone(), w.grad.clone()
+    x.grad = w.grad = None
+    (ssm.causal_conv(x, w, time_major=False).transpose(1, 2) * torch.ones(2, 6, 9, device="cuda")).sum().backward()
+    assert torch.equal(a[0], x.grad) and torch.equal(a[1], w.grad)
+
+
+def test_long_sequences_and_many_of_them():
+    """A sequence of 20000 steps (chunks of the time axis), and 70000 of two (more than a grid's other dimensions hold),
+    against the same rows one by one."""
+    g = torch.Generator().manual_seed(2)
+    rnd = lambda *s: torch.randn(s, generator=g).cuda()                                           # noqa: E731
+    A = -torch.rand(8, 4, generator=g).cuda()
+    x, d, B, C = rnd(1, 20000, 8), rnd(1, 20000, 8), rnd(1, 20000, 4), rnd(1, 20000, 4)
+    y, end, tape = ssm.selective_scan_train(x, d, A, B, C, want_final_state=True, time_major=False)
+    state, ys = None, []
+    for t in range(0, 20000, 5000):
+        p, state = ssm.selective_scan_forward(x[:, t:t + 5000], d[:, t:t + 5000], A, B[:, t:t + 5000], C[:, t:t + 5000], initial_state=state,
+                                              want_final_state=True, time_major=False)
+        ys.append(p)
+    # decays of at least exp(-s A) forget: what differs is the last few hundred steps' rounding
+    assert float((torch.cat(ys, 1) - y).abs().max()) <= 1000 * R.EPS32 * float(y.abs().max())
+    assert float((state - end).abs().max()) <= 1000 * R.EPS32 * float(end.abs().max())
+    gr = ssm.selective_scan_backward(x, d, A, B, C, torch.ones_like(y), tape, time_major=False)
+    assert all(torch.isfinite(t).all() for t in gr if t is not None)
+    many = [rnd(2, 70000, 8), rnd(2, 70000, 8), A, rnd(2, 70000, 4), rnd(2, 70000, 4)]
+    y, _, tape = ssm.selective_scan_train(*many)
+    gr = ssm.selective_scan_backward(*many, torch.ones_like(y), tape)
+    part = [t[:, 69990:] if t is not A else A for t in many]
+    y1, _, tape1 = ssm.selective_scan_train(*part)
+    g1 = ssm.selective_scan_backward(*part, torch.ones_like(y1), tape1)
+    assert torch.equal(y[:, 69990:], y1) and torch.equal(gr.dx[:, 69990:], g1.dx) and torch.equal(gr.dB[:, 69990:], g1.dB)
+    assert torch.equal(ssm.causal_conv_forward(many[0], rnd(8, 4))[0].isfinite().all(), torch.tensor(True, device="cuda"))
