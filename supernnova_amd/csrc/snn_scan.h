@@ -34,6 +34,7 @@ template <typename T> struct ScanP {
     float *carry, *csum;                // split over time: state (adjoint) entering chunk c, and the sum of steps of chunk c
     int D, N, dg, cbg, softplus;        // channels, states, channels per group, channel blocks per group
     int tc, nc;                         // steps per chunk, chunks
+    const int* order;                   // sequences, longest first, or NULL
     int vec;                            // rows of N states start at multiples of 16 bytes and fill the lanes
     // backward
     View<T> dy, dx, ddelta, dz, dB, dC;
@@ -182,5 +183,7 @@ template <typename T> __device__ __forceinline__ void clear_channels(const View<
 int snn_scan_check(const snn_scan_args* a, const char* fn);
 struct ScanGrid { int cbg, blocks_c, tc, nc; };
 ScanGrid snn_scan_grid(const snn_scan_args* a);
+bool snn_scan_ordered(const snn_scan_args* a, const ScanGrid& g);
+void snn_scan_launch_order(const snn_seq& seq, int* order, hipStream_t s);
 template <typename T> ScanP<T> scan_params(const snn_scan_args* a, const ScanGrid& g);
 void snn_scan_launch_combine(const snn_scan_args* a, const ScanGrid& g, const float* edge, float* carry, const float* csum, bool reverse, hipStream_t s);

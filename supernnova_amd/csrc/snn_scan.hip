@@ -24,7 +24,8 @@ template <typename T, int K, int LN, bool STATE_ONLY, bool GATE> __global__ void
 {
     constexpr int SEG = SCAN_SEG, G = SEG / 4, TS = ScanTape<K>::STEPS, NP = K * LN, CH = 256 / LN;
     __shared__ float sB[2][SEG * NP], sC[2][STATE_ONLY ? 1 : SEG * NP];
-    const int tid = threadIdx.x, b = blockIdx.x, cb = blockIdx.y, c = blockIdx.z;
+    const int tid = threadIdx.x, c = blockIdx.z;
+    const int b = p.order ? p.order[blockIdx.y] : blockIdx.x, cb = p.order ? blockIdx.x : blockIdx.y;
     const ScanCh ch = scan_channel<K, LN>(cb, p.cbg, p.dg, tid);
     const int j = ch.j, d = ch.d;
     const SeqRange r = seq_range(p.seq, b);
@@ -143,6 +144,24 @@ template <typename T, int K, int LN, bool STATE_ONLY, bool GATE> __global__ void
     const int left = p.dg - (cb - ch.g * p.cbg) * CH;
     clear_channels(p.y, r.row0 * p.y.st + b * p.y.sb, fill_range(p.seq, r, b, t0, t0 + p.tc, c == p.nc - 1), ch.g * p.dg + p.dg - left,
                    left < CH ? left : CH, tid);
+}
+
+// order[r] = the sequence of rank r by length, longest first, equal ones by index: workgroups are dealt longest first, so that the
+// last ones to run are short.  A wave counts the sequences in front of its own.
+__global__ void __launch_bounds__(256) scan_order_kernel(const snn_seq seq, int* order)
+{
+    const int b = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (b >= seq.n_seq) return;
+    const int len = seq_range(seq, b).len;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = lane; j < seq.n_seq; j += 64) {
+        const int l = seq_range(seq, j).len;
+        rank += l > len || (l == len && j < b);
+    }
+#pragma unroll
+    for (int m = 32; m; m >>= 1) rank += __shfl_xor(rank, m);
+    if (lane == 0) order[rank] = b;
 }
 
 // carry[b][c] from the chunks' local results, over the chunks of a sequence.  Forward: slot c holds chunk c-1's local last
@@ -265,6 +284,17 @@ ScanGrid snn_scan_grid(const snn_scan_args* a)
     return g;
 }
 
+// Longest first pays where the grid runs in a few rounds (512 workgroups and more, one chunk a sequence) over sequences of different
+// lengths; beyond 4096 sequences the rounds are many and even out, and the ranks would cost more than they give.
+bool snn_scan_ordered(const snn_scan_args* a, const ScanGrid& g)
+{
+    return (a->seq.lengths || a->seq.offsets) && (int64_t)g.blocks_c * a->seq.n_seq >= 512 && a->seq.n_seq > 1 && a->seq.n_seq <= 4096;
+}
+void snn_scan_launch_order(const snn_seq& seq, int* order, hipStream_t s)
+{
+    hipLaunchKernelGGL(scan_order_kernel, dim3((unsigned)((seq.n_seq + 3) / 4)), dim3(256), 0, s, seq, order);
+}
+
 template <typename T> ScanP<T> scan_params(const snn_scan_args* a, const ScanGrid& g)
 {
     ScanP<T> p;
@@ -305,6 +335,7 @@ template <typename T> ScanP<T> scan_params(const snn_scan_args* a, const ScanGri
     p.dh0 = a->dstate_in;
     p.part = p.bcpart = nullptr;
     p.slots = 0;
+    p.order = nullptr;
     return p;
 }
 template ScanP<float> scan_params<float>(const snn_scan_args*, const ScanGrid&);
@@ -322,8 +353,13 @@ void snn_scan_launch_combine(const snn_scan_args* a, const ScanGrid& g, const fl
 namespace {
 template <typename T, int K, int LN> int forward(const snn_scan_args* a, const ScanGrid& g, hipStream_t s)
 {
-    const ScanP<T> p = scan_params<T>(a, g);
-    const dim3 grid((unsigned)a->seq.n_seq, (unsigned)g.blocks_c, (unsigned)g.nc);
+    ScanP<T> p = scan_params<T>(a, g);
+    dim3 grid((unsigned)a->seq.n_seq, (unsigned)g.blocks_c, (unsigned)g.nc);
+    if (snn_scan_ordered(a, g)) {
+        snn_scan_launch_order(a->seq, (int*)a->ws, s);
+        p.order = (const int*)a->ws;
+        std::swap(grid.x, grid.y);
+    }
     if (g.nc > 1) {
         hipLaunchKernelGGL((scan_fwd_kernel<T, K, LN, true, false>), grid, dim3(256), 0, s, p);
         snn_scan_launch_combine(a, g, a->state_in, p.carry, p.csum, false, s);

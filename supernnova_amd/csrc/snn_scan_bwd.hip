@@ -161,7 +161,7 @@ template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds_
     float* bcpart = p.bcpart ? p.bcpart + (int64_t)cb * rows * (2 * NP) : nullptr;
     const int items = p.seq.n_seq * p.nc;
     for (int item = slot; item < items; item += p.slots) {
-        const int b = item / p.nc, c = item - b * p.nc;
+        const int bi = item / p.nc, c = item - bi * p.nc, b = p.order ? p.order[bi] : bi;
         const SeqRange r = seq_range(p.seq, b);
         const int t0 = c * p.tc, t1 = t0 + p.tc < r.len ? t0 + p.tc : r.len;
         const int64_t rowb = p.seq.offsets ? r.row0 : (int64_t)b * p.seq.max_T;
@@ -399,7 +399,7 @@ template <typename T> __global__ void __launch_bounds__(256) scan_bc_sum_kernel(
         if (n + i < p.N) out[i] = from_f32<T>(v[i]);
 }
 
-struct Sizes { int64_t carry, csum, part, bc; int slots; };
+struct Sizes { int64_t carry, csum, order, part, bc; int slots; };
 // Slots: workgroups that share the chunks.  2048 of them all told keep four on every compute unit in turn and even out
 // ragged lengths; more would only add partial sums to write and read.
 Sizes sizes(const snn_scan_args* a, const ScanGrid& g)
@@ -410,6 +410,7 @@ Sizes sizes(const snn_scan_args* a, const ScanGrid& g)
     z.slots = (int)std::min<int64_t>(items, std::max<int64_t>(1, 2048 / g.blocks_c));
     z.carry = g.nc > 1 ? items * a->channels * NP : 0;
     z.csum = g.nc > 1 ? (items * a->channels + 3) / 4 * 4 : 0;
+    z.order = snn_scan_ordered(a, g) ? ((int64_t)a->seq.n_seq + 3) / 4 * 4 : 0;
     z.part = (int64_t)z.slots * part_stride(a->channels, NP);
     const int64_t rows = a->seq.offsets ? a->seq.n_rows : (int64_t)a->seq.n_seq * a->seq.max_T;
     z.bc = g.cbg > 1 ? (int64_t)g.blocks_c * rows * 2 * NP : 0;
@@ -422,7 +423,11 @@ template <typename T, int K, int LN, bool GATE> int backward(const snn_scan_args
     const Sizes z = sizes(a, g);
     p.carry = (float*)a->ws;
     p.csum = p.carry + z.carry;
-    p.part = p.csum + z.csum;
+    p.part = p.csum + z.csum + z.order;
+    if (z.order) {
+        snn_scan_launch_order(a->seq, (int*)(p.part - z.order), s);
+        p.order = (const int*)(p.part - z.order);
+    }
     p.bcpart = z.bc ? p.part + z.part : nullptr;
     p.slots = z.slots;
     if (g.nc > 1) {
@@ -462,7 +467,7 @@ extern "C" int64_t snn_scan_workspace_bytes(const snn_scan_args* a, int32_t back
     if (int rc = snn_scan_check(a, "snn_scan_workspace_bytes")) return rc;
     const ScanGrid g = snn_scan_grid(a);
     const Sizes z = sizes(a, g);
-    return 4 * (z.carry + z.csum + (backward_pass ? z.part + z.bc : 0));
+    return 4 * (z.carry + z.csum + z.order + (backward_pass ? z.part + z.bc : 0));
 }
 
 extern "C" int snn_scan_backward(const snn_scan_args* a, void* stream)

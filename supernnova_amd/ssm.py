@@ -236,9 +236,10 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_stat
 
 # ------------------------------------------------------------------------------------------------- scan
 @functools.lru_cache(maxsize=256)
-def _scan_sizes(dtype, D, N, G, B, T, rows, ragged):
-    """(tape floats, forward workspace bytes, backward workspace bytes): they depend on the sizes alone."""
-    a = L.SnnScanArgs(seq=L.SnnSeq(B, T, rows, None, 8 if ragged else None), dtype=dtype, channels=D, states=N, groups=G)
+def _scan_sizes(dtype, D, N, G, B, T, rows, lengths, offsets):
+    """(tape floats, forward workspace bytes, backward workspace bytes): they depend on the sizes, and on whether there are lengths
+    or offsets (the addresses are not looked at)."""
+    a = L.SnnScanArgs(seq=L.SnnSeq(B, T, rows, 8 if lengths else None, 8 if offsets else None), dtype=dtype, channels=D, states=N, groups=G)
     lib, p = L.load(), ctypes.byref(a)
     return (L.check(lib.snn_scan_tape_floats(p), "snn_scan_tape_floats"), L.check(lib.snn_scan_workspace_bytes(p, 0), "snn_scan_workspace_bytes"),
             L.check(lib.snn_scan_workspace_bytes(p, 1), "snn_scan_workspace_bytes"))
@@ -272,7 +273,7 @@ def _scan_forward(x, delta, A, B, C, D, z, delta_bias, delta_softplus, lengths, 
     y, vy = bt.empty()
     head, G, N, _ = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, vy)
     state = bt.param(initial_state, "initial_state", (bt.B, bt.D, N))
-    n_tape, need, _ = _scan_sizes(head[5], bt.D, N, G, bt.B, bt.T, bt.seq[2], offsets is not None)
+    n_tape, need, _ = _scan_sizes(head[5], bt.D, N, G, bt.B, bt.T, bt.seq[2], lengths is not None, offsets is not None)
     end = bt.floats(bt.B, bt.D, N) if want_final_state else None
     tape = bt.floats(n_tape) if want_tape else None
     ws = bt.floats(need // 4) if need else None
@@ -306,7 +307,7 @@ def selective_scan_backward(x, delta, A, B, C, dy, tape, D=None, z=None, delta_b
     head, G, N, shape = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, _NO_VIEW)
     dy, Dm, sizes = _unit(dy), bt.D, (bt.B, bt.D, N)
     vdy, state, dend = bt.view(dy, "dy"), bt.param(initial_state, "initial_state", sizes), bt.param(dfinal_state, "dfinal_state", sizes)
-    n_tape, _, need = _scan_sizes(head[5], Dm, N, G, bt.B, bt.T, bt.seq[2], offsets is not None)
+    n_tape, _, need = _scan_sizes(head[5], Dm, N, G, bt.B, bt.T, bt.seq[2], lengths is not None, offsets is not None)
     if tape.numel() < n_tape:
         _fail(f"the tape is too small: {tape.numel()} floats, {n_tape} needed (of selective_scan_train over the same inputs)")
     tape_p = bt.param(tape, "tape", tape.shape)

@@ -174,6 +174,10 @@ SCAN = [  # dt, layout, D, N, G, lens, gate, state, strided
     ("f32", "time", 200, 24, 2, (260, 257), False, True, True),
 ]
 
+# enough workgroups for the sequences to be taken longest first
+_MANY = tuple(int(v) for v in np.random.default_rng(0).integers(0, 14, 200))
+SCAN += [("f32", "time", 130, 16, 1, _MANY, True, True, False), ("bf16", "rows", 150, 4, 1, _MANY, False, True, False)]
+
 
 @pytest.mark.parametrize("dt,layout,D,N,G,lens,gate,state,strided", SCAN)
 def test_scan(dt, layout, D, N, G, lens, gate, state, strided):
