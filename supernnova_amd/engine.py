@@ -548,37 +548,38 @@ def _clip(tensors, max_norm, norm_type, grad_scale, out):
     if dev.type != "cuda":
         raise L.SnnError("gradients must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")
     # whole-list passes: a model has hundreds of gradients, and a line of Python for each costs more than its share of the kernel
+    n, types = len(src), [t.dtype for t in src]
     try:
-        dts = [_DTYPES[t.dtype] for t in src]
+        dts = [_DTYPES[types[0]]] * n if types.count(types[0]) == n else [_DTYPES[d] for d in types]
     except KeyError as e:
         raise L.SnnError(f"gradients of type {e.args[0]}: supported are float32, bfloat16 and float16") from None
     whole = all([t.is_contiguous() for t in src])
-    if [t.get_device() for t in src].count(dev.index) != len(src) or not (whole or all(_dense(t) for t in src)):
+    if [t.get_device() for t in src].count(dev.index) != n or not (whole or all(_dense(t) for t in src)):
         raise L.SnnError("gradients must be dense tensors (no gaps, no repeated elements) on one device")
-    n = len(src)
     numel = array.array("q", [t.numel() for t in src])
     ptrs = array.array("Q", [t.data_ptr() for t in src])
     dst = None
     if out is not None:
-        if len(set(ptrs)) != n:
-            full = [p for p, k in zip(ptrs, numel) if k]
-            if len(set(full)) != len(full):
-                raise L.SnnError("a gradient is listed twice")
+        apart = set(ptrs)
+        if len(apart) != n and len({p for p, k in zip(ptrs, numel) if k}) != sum(map(bool, numel)):
+            raise L.SnnError("a gradient is listed twice")
         if out is src:
             dst = ptrs
         else:
             out = list(out)
             if len(out) != n:
                 raise L.SnnError(f"out has {len(out)} tensors for {n} gradients")
-            if [o.shape for o in out] != [t.shape for t in src] or [o.dtype for o in out] != [t.dtype for t in src] or \
+            if [o.dtype for o in out] != types or array.array("q", [o.numel() for o in out]) != numel or \
                     [o.get_device() for o in out].count(dev.index) != n or \
-                    not (whole and all([o.is_contiguous() for o in out]) or [o.stride() for o in out] == [t.stride() for t in src]):
-                raise L.SnnError("out must match the gradients in shape, strides, type and device")
+                    not (whole and all([o.is_contiguous() for o in out]) or
+                         [(o.shape, o.stride()) for o in out] == [(t.shape, t.stride()) for t in src]):
+                raise L.SnnError("out must match the gradients in elements, strides, type and device")
             dst = array.array("Q", [o.data_ptr() for o in out])
-            full = [(d, s) for d, s, k in zip(dst, ptrs, numel) if k]
-            apart = {d for d, s in full}
-            if len(apart) != len(full) or any(s in apart and s != d for d, s in full):
-                raise L.SnnError("out lists a tensor twice, or the place of another gradient")
+            if len(set(dst)) != n or not apart.isdisjoint(dst):
+                pairs = [(d, s) for d, s, k in zip(dst, ptrs, numel) if k]
+                to = {d for d, s in pairs}
+                if len(to) != len(pairs) or any(s in to and s != d for d, s in pairs):
+                    raise L.SnnError("out lists a tensor twice, or the place of another gradient")
     lib = L.load()
     dts = array.array("i", dts)
     at = numel.buffer_info()[0]
@@ -598,8 +599,8 @@ def grad_norm(tensors, norm_type=2.0):
 
 
 def clip_grads(tensors, max_norm, norm_type=2.0, out=None):
-    """Multiply every gradient by min(1, max_norm / (norm + 1e-6)), in place, or into `out` (a list of tensors like them);
-    returns the norm from before as a 0-dim fp32 device tensor.  Gradients that are not finite are not looked for: a norm of
+    """Multiply every gradient by min(1, max_norm / (norm + 1e-6)), in place, or into `out`, a list of tensors like them
+    (contiguous ones may have another shape: slices of a flat buffer); returns the norm from before as a 0-dim fp32 device tensor.  Gradients that are not finite are not looked for: a norm of
     inf gives 0 (and NaN where a gradient is inf), a norm of NaN gives NaN, as torch.nn.utils.clip_grad_norm_."""
     tensors = list(tensors)
     return _clip(tensors, float(max_norm), norm_type, 1.0, tensors if out is None else out)[0]

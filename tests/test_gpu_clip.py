@@ -104,6 +104,11 @@ def test_dense_orders_and_refusals():
         E.clip_grads([t], 1.0, out=[t.half()])
     with pytest.raises(L.SnnError, match="out"):
         E.clip_grads([t], 1.0, out=[torch.empty(5, 6, device="cuda").t()])
+    with pytest.raises(L.SnnError, match="out"):
+        E.clip_grads([t], 1.0, out=[torch.empty(29, device="cuda")])
+    flat = torch.empty(30, device="cuda")
+    E.clip_grads([t], 1.0, out=[flat])
+    assert abs(float(flat.double().norm()) - 1.0) <= 2e-6 and torch.equal(flat.sign(), t.sign().reshape(-1))
     with pytest.raises(L.SnnError, match="out has"):
         E.clip_grads([t], 1.0, out=[])
     with pytest.raises(L.SnnError, match="twice"):
