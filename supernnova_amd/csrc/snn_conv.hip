@@ -11,6 +11,7 @@
 #include "snn_seq.h"
 #include "snn_host.h"
 #include <algorithm>
+#include <type_traits>
 
 #define HIP_CHECK(x) do { hipError_t e_ = (x); if (e_ != hipSuccess) { \
     snn_set_error("%s: %s", #x, hipGetErrorString(e_)); return SNN_ERR_HIP; } } while (0)
@@ -152,64 +153,78 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
             for (int k = 0; k < W; ++k) zero_v(dpw[k]);
             constexpr int U = 4;
             const int te = t1 + W - 1;              // dx of the chunk's last step needs the W - 1 steps behind it
-            for (int tb = t0; tb < te; tb += U) {
+            const T *xp = p.x.p + xb + t0 * p.x.st, *gp = p.dy.p + gb + t0 * p.dy.st;
+            T* op = p.dx.p + ob + (t0 - (W - 1)) * p.dx.st;
+            // steps tb .. tb + 3.  INNER: all of them are the chunk's, and so are the steps W - 1 before them, whose gradients
+            // they complete: nothing to ask.
+            auto group = [&](auto inner, int tb) {
+                constexpr bool INNER = decltype(inner)::value;
                 Pack<T, V> rx[U], rg[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if (tb + u < r.len && tb + u < te) {
-                        rx[u] = *(const Pack<T, V>*)(p.x.p + xb + (tb + u) * p.x.st);
-                        rg[u] = *(const Pack<T, V>*)(p.dy.p + gb + (tb + u) * p.dy.st);
+                    if (INNER || (tb + u < r.len && tb + u < te)) {
+                        rx[u] = *(const Pack<T, V>*)(xp + u * p.x.st);
+                        rg[u] = *(const Pack<T, V>*)(gp + u * p.dy.st);
                     }
                 }
+                xp += U * p.x.st;
+                gp += U * p.dy.st;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int t = tb + u;
-                    if (t < te) {
-                        const bool live = t < r.len;
-                        float out[V];
+                    if (!INNER && t >= te) break;
+                    const bool live = INNER || t < r.len, ours = INNER || t < t1;
+                    float out[V];
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            float dp = 0.0f;
-                            win[W - 1][i] = 0.0f;
-                            if (live) {
-                                win[W - 1][i] = to_f32(rx[u].v[i]);
-                                float a = bs[i];
+                    for (int i = 0; i < V; ++i) {
+                        float dp = 0.0f;
+                        win[W - 1][i] = 0.0f;
+                        if (live) {
+                            win[W - 1][i] = to_f32(rx[u].v[i]);
+                            float a = bs[i];
 #pragma unroll
-                                for (int k = 0; k < W; ++k) a = fmaf(wt[k][i], win[k][i], a);
-                                dp = to_f32(rg[u].v[i]);
-                                if (p.silu) {
-                                    const float s = sigmoid_f32(a);
-                                    dp *= s * fmaf(a, 1.0f - s, 1.0f);
-                                }
-                                if (t < t1) {
-#pragma unroll
-                                    for (int k = 0; k < W; ++k) dw[k][i] = fmaf(dp, win[k][i], dw[k][i]);
-                                    db[i] += dp;
-                                }
+                            for (int k = 0; k < W; ++k) a = fmaf(wt[k][i], win[k][i], a);
+                            dp = to_f32(rg[u].v[i]);
+                            if (p.silu) {
+                                const float s = sigmoid_f32(a);
+                                dp *= s * fmaf(a, 1.0f - s, 1.0f);
                             }
+                            if (ours) {
 #pragma unroll
-                            for (int k = W - 1; k > 0; --k) dpw[k][i] = dpw[k - 1][i];
-                            dpw[0][i] = dp;
-                            out[i] = 0.0f;
-#pragma unroll
-                            for (int k = 0; k < W; ++k) out[i] = fmaf(wt[k][i], dpw[k][i], out[i]);
-#pragma unroll
-                            for (int k = 0; k < W - 1; ++k) win[k][i] = win[k + 1][i];
+                                for (int k = 0; k < W; ++k) dw[k][i] = fmaf(dp, win[k][i], dw[k][i]);
+                                db[i] += dp;
+                            }
                         }
-                        const int tau = t - (W - 1);            // the step whose gradient is complete now
-                        const int k = tau - r.len + W - 1;      // its place among the last W - 1 inputs
-                        const bool ours = tau >= t0 || (c == 0 && tau < 0);
-                        if (ours && p.ds_out && k >= 0 && k < W - 1) {
+#pragma unroll
+                        for (int k = W - 1; k > 0; --k) dpw[k][i] = dpw[k - 1][i];
+                        dpw[0][i] = dp;
+                        out[i] = wt[0][i] * dp;
+#pragma unroll
+                        for (int k = 1; k < W; ++k) out[i] = fmaf(wt[k][i], dpw[k][i], out[i]);
+#pragma unroll
+                        for (int k = 0; k < W - 1; ++k) win[k][i] = win[k + 1][i];
+                    }
+                    const int tau = t - (W - 1);            // the step whose gradient is complete now
+                    if (INNER) store_v<T, V>(op + u * p.dx.st, out);
+                    else {
+                        const int k = tau - r.len + W - 1;  // its place among the last W - 1 inputs
+                        const bool mine = tau >= t0 || (c == 0 && tau < 0);
+                        if (mine && p.ds_out && k >= 0 && k < W - 1) {
                             float e[V];
                             load_v<T, V>(p.ds_out + ((int64_t)b * (W - 1) + k) * p.D + d, e);
 #pragma unroll
                             for (int i = 0; i < V; ++i) out[i] += e[i];
                         }
-                        if (tau >= t0) store_v<T, V>(p.dx.p + ob + tau * p.dx.st, out);
-                        else if (ours && p.ds_in) store_v<T, V>(p.ds_in + ((int64_t)b * (W - 1) + (tau + W - 1)) * p.D + d, out);
+                        if (tau >= t0) store_v<T, V>(op + u * p.dx.st, out);
+                        else if (mine && p.ds_in) store_v<T, V>(p.ds_in + ((int64_t)b * (W - 1) + (tau + W - 1)) * p.D + d, out);
                     }
                 }
-            }
+                op += U * p.dx.st;
+            };
+            int tb = t0;
+            group(std::false_type{}, tb);           // the first W - 1 <= U steps complete the chunk's (or the state's) before
+            for (tb += U; tb + U <= t1; tb += U) group(std::true_type{}, tb);
+            for (; tb < te; tb += U) group(std::false_type{}, tb);
         }
         clear_rows<T, V>(p.dx, fill_range(p.seq, r, b, t0, t0 + p.tc, c == p.nc - 1), ob);
     }
@@ -276,6 +291,7 @@ int check_args(const snn_conv_args* a, int what, const char* fn)
     return SNN_OK;
 }
 // 16 bytes of a row per thread (backward: 4 channels) where every row starts at a multiple of that, one channel otherwise.
+// 8192 x 4096 bf16: forward 27.5 us against 31.5 with one channel a thread, backward 48.5 against 59.
 int vector_width(const snn_conv_args* a, int what)
 {
     const int e = ELEM[a->dtype], v = what == BWD ? 4 : 16 / e;
