@@ -134,11 +134,11 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= (int64_t)p.slots * p.cv) return;
     const int slot = (int)(id / p.cv), d = (int)(id - (int64_t)slot * p.cv) * V;
-    float wt[W][V], bs[V], dw[W][V], db[V];
+    float wt[W][V], bs[V], dws[W][V], dbs[V];     // sums over the chunks; a chunk's own come first, so that long sums stay exact
     load_taps<V, W>(p.weight, p.bias, d, wt, bs);
-    zero_v(db);
+    zero_v(dbs);
 #pragma unroll
-    for (int k = 0; k < W; ++k) zero_v(dw[k]);
+    for (int k = 0; k < W; ++k) zero_v(dws[k]);
     for (int64_t item = slot; item < p.items; item += p.slots) {
         const int b = (int)(item / p.nc), c = (int)(item - (int64_t)b * p.nc);
         const SeqRange r = seq_range(p.seq, b);
@@ -146,7 +146,10 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
         const int64_t xb = r.row0 * p.x.st + b * p.x.sb + d, gb = r.row0 * p.dy.st + b * p.dy.sb + d;
         const int64_t ob = r.row0 * p.dx.st + b * p.dx.sb + d;
         if (t0 < t1 || c == 0) {                    // c == 0: the gradient of the initial state, also of an empty sequence
-            float win[W][V], dpw[W][V];             // dpw[k] = dp of k steps ago
+            float win[W][V], dpw[W][V], dw[W][V], db[V];             // dpw[k] = dp of k steps ago
+            zero_v(db);
+#pragma unroll
+            for (int k = 0; k < W; ++k) zero_v(dw[k]);
 #pragma unroll
             for (int k = 0; k < W - 1; ++k) load_before<T, V, W>(p, xb, b, t0 - (W - 1) + k, d, win[k]);
 #pragma unroll
@@ -225,6 +228,12 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
             group(std::false_type{}, tb);           // the first W - 1 <= U steps complete the chunk's (or the state's) before
             for (tb += U; tb + U <= t1; tb += U) group(std::true_type{}, tb);
             for (; tb < te; tb += U) group(std::false_type{}, tb);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+#pragma unroll
+                for (int k = 0; k < W; ++k) dws[k][i] += dw[k][i];
+                dbs[i] += db[i];
+            }
         }
         clear_rows<T, V>(p.dx, fill_range(p.seq, r, b, t0, t0 + p.tc, c == p.nc - 1), ob);
     }
@@ -232,8 +241,8 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) q[k * p.D + i] = dw[k][i];
-        q[W * p.D + i] = db[i];
+        for (int k = 0; k < W; ++k) q[k * p.D + i] = dws[k][i];
+        q[W * p.D + i] = dbs[i];
     }
 }
 

@@ -149,12 +149,12 @@ template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds_
     const ScanCh ch = scan_channel<K, LN>(cb, p.cbg, p.dg, tid);
     const int j = ch.j, d = ch.d;
     const int left_ch = p.dg - (cb - ch.g * p.cbg) * CH, d0 = ch.g * p.dg + p.dg - left_ch;
-    float A2[K], dA[K], dsk = 0.0f, dbs = 0.0f;
+    float A2[K], dAs[K], dsks = 0.0f, dbss = 0.0f;      // sums over blocks of 256 steps; a block's own come first, so that long sums stay exact
     load_states<K>(p.A + (int64_t)d * p.N, ch.n, p.N, p.vec, A2);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         A2[k] *= SNN_LOG2E;
-        dA[k] = 0.0f;
+        dAs[k] = 0.0f;
     }
     const float bias = p.dbias ? p.dbias[d] : 0.0f, skip = p.skip ? p.skip[d] : 0.0f;
     const int64_t rows = p.seq.offsets ? p.seq.n_rows : (int64_t)p.seq.n_seq * p.seq.max_T;
@@ -165,9 +165,9 @@ template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds_
         const SeqRange r = seq_range(p.seq, b);
         const int t0 = c * p.tc, t1 = t0 + p.tc < r.len ? t0 + p.tc : r.len;
         const int64_t rowb = p.seq.offsets ? r.row0 : (int64_t)b * p.seq.max_T;
-        float w[K];                                               // a_{t+1} q_{t+1}
+        float w[K], dA[K], dsk = 0.0f, dbs = 0.0f;                // w: a_{t+1} q_{t+1}
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k] = 0.0f;
+        for (int k = 0; k < K; ++k) w[k] = dA[k] = 0.0f;
         if (p.nc > 1 && t0 < r.len) load_states<K>(p.carry + (((int64_t)b * p.nc + c) * p.D + d) * NP, ch.n, NP, true, w);
         else if (c == 0 && p.dhT) load_states<K>(p.dhT + ((int64_t)b * p.D + d) * p.N, ch.n, p.N, p.vec, w);
         if (t0 < t1) {
@@ -304,6 +304,16 @@ template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds_
                         dsk = fmaf(g[i], x[i], dsk);
                     }
                 }
+                if (t % 256 == 0 || t == t0) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        dAs[k] += dA[k];
+                        dA[k] = 0.0f;
+                    }
+                    dsks += dsk;
+                    dbss += dbs;
+                    dsk = dbs = 0.0f;
+                }
                 dxp -= SEG * p.dx.st;
                 ddp -= SEG * p.ddelta.st;
                 if (GATE) dzp -= SEG * p.dz.st;
@@ -336,14 +346,14 @@ template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds_
             clear_channels(p.dC, r.row0 * p.dC.st + b * p.dC.sb + ch.g * p.N, f, 0, p.N, tid);
         }
     }
-    dsk = quad_sum(dsk);
-    dbs = quad_sum(dbs);
+    dsks = quad_sum(dsks);
+    dbss = quad_sum(dbss);
     if (ch.ok) {
         float* q = p.part + (int64_t)slot * part_stride(p.D, NP);
-        store_states<K>(q + (int64_t)d * NP, ch.n, NP, true, dA);
+        store_states<K>(q + (int64_t)d * NP, ch.n, NP, true, dAs);
         if (ch.n == 0) {
-            q[(int64_t)p.D * NP + d] = dsk;
-            q[(int64_t)p.D * (NP + 1) + d] = dbs;
+            q[(int64_t)p.D * NP + d] = dsks;
+            q[(int64_t)p.D * (NP + 1) + d] = dbss;
         }
     }
 }
