@@ -452,6 +452,7 @@ int snn_train_step_grad(const snn_cfg *cfg, const snn_train_io *io, void *stream
  * elements, in any alignment.
  *   norm = grad_scale (sum |g|^p)^(1/p), norm_type 1, 2, or 0 for the largest magnitude;  coef = min(1, max_norm / (norm + 1e-6))
  *   out[0] = norm, out[1] = coef (device floats);  dst[i] = src[i] * coef if dst != NULL (dst[i] may be src[i])
+ * A dst[i] that overlaps another one, or a gradient other than src[i], is refused.
  * Sums are fp64 in an order that depends on the sizes alone.  Not finite gradients give the norm and the products IEEE
  * arithmetic gives.  scratch: snn_clip_scratch_doubles(n_tensors, numel) doubles.
  * grad_scale: what the optimizer will multiply gradients by (1 / world size after a data-parallel sum).
@@ -486,7 +487,8 @@ int snn_sgd_step_clipped(int64_t n, float *params, const float *grads, float *mo
  * [offsets[b], offsets[b + 1]) (n_seq + 1 entries, DEVICE), none longer than max_T.  The device arrays are read by the
  * kernels only; values out of range are cut to the tensors (a length to [0, max_T], an offset to [0, n_rows]).
  * Rows that belong to no step -- behind a sequence's end in a padded batch, outside every sequence among ragged rows, past
- * max_T -- are never read, and zero in every output.  A sequence of length 0 hands its initial state on.
+ * max_T -- are never read, and zero in every output.  A sequence of length 0 hands its initial state on.  Offsets must not
+ * decrease (rows that two sequences share have no defined result).  At most 2^24 - 1 sequences, 2^30 steps, 2^19 channels.
  */
 typedef struct snn_seq {
     int32_t n_seq, max_T;

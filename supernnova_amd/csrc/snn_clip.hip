@@ -10,6 +10,9 @@
 // single workgroup does it in between.
 #include <hip/hip_runtime.h>
 #include <math.h>
+#include <algorithm>
+#include <memory>
+#include <new>
 #include "snn_host.h"
 #include "snn_seq.h"
 
@@ -253,6 +256,41 @@ void run(int n_tensors, const void* const* src, void* const* dst, const int64_t*
         });
 }
 
+// Results may not share memory with each other, nor with any gradient but their own (which they must then cover exactly): the
+// workgroups of two tensors run at once.
+struct Span { uintptr_t lo, hi; int i; };
+int check_apart(int n_tensors, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype)
+{
+    auto bytes = [&](int i) { return (uintptr_t)numel[i] * (dtype[i] == SNN_DT_F32 ? 4 : 2); };
+    const std::unique_ptr<Span[]> to(new (std::nothrow) Span[n_tensors + 1]);
+    if (!to) { snn_set_error("snn_clip_grads: out of host memory"); return SNN_ERR_ARG; }
+    int n = 0;
+    bool in_place = true;
+    for (int i = 0; i < n_tensors; ++i) {
+        if (!numel[i]) continue;
+        to[n++] = Span{(uintptr_t)dst[i], (uintptr_t)dst[i] + bytes(i), i};
+        in_place = in_place && dst[i] == src[i];
+    }
+    std::sort(to.get(), to.get() + n, [](const Span& a, const Span& b) { return a.lo < b.lo; });
+    for (int k = 1; k < n; ++k)
+        if (to[k].lo < to[k - 1].hi) {
+            snn_set_error("snn_clip_grads: a gradient or a place in out is listed twice, or two of them overlap (tensors %d, %d)", to[k - 1].i, to[k].i);
+            return SNN_ERR_ARG;
+        }
+    for (int i = 0; i < n_tensors && !in_place; ++i) {
+        if (!numel[i]) continue;
+        const uintptr_t lo = (uintptr_t)src[i], hi = lo + bytes(i);
+        // the first result that ends behind lo, and those that begin before hi
+        const Span* s = std::upper_bound(to.get(), to.get() + n, lo, [](uintptr_t v, const Span& a) { return v < a.hi; });
+        for (; s < to.get() + n && s->lo < hi; ++s)
+            if (s->i != i || s->lo != lo) {
+                snn_set_error("snn_clip_grads: out overlaps another gradient, or its own in part (tensors %d, %d)", s->i, i);
+                return SNN_ERR_ARG;
+            }
+    }
+    return SNN_OK;
+}
+
 }  // namespace
 
 extern "C" int64_t snn_clip_scratch_doubles(int32_t n_tensors, const int64_t* numel)
@@ -285,6 +323,8 @@ extern "C" int snn_clip_grads(int32_t n_tensors, const void* const* src, void* c
             snn_set_error("snn_clip_grads: tensor %d: null pointer or dtype %d", i, dtype[i]);
             return SNN_ERR_ARG;
         }
+    if (dst)
+        if (int rc = check_apart(n_tensors, src, dst, numel, dtype)) return rc;
     const hipStream_t s = (hipStream_t)stream;
     if (norm_type == 2) run<2>(n_tensors, src, dst, numel, dtype, max_norm, grad_scale, out, scratch, pieces, s);
     else if (norm_type == 1) run<1>(n_tensors, src, dst, numel, dtype, max_norm, grad_scale, out, scratch, pieces, s);

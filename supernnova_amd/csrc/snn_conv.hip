@@ -296,6 +296,10 @@ int check_args(const snn_conv_args* a, int what, const char* fn)
         snn_set_error("%s: dtype %d / width %d: supported are dtypes 0..2 (SNN_DT_*) and 2..4 taps", fn, a->dtype, a->width);
         return SNN_ERR_UNSUPPORTED;
     }
+    if (!snn_sizes_fit(a->seq, a->channels)) {
+        snn_set_error("%s: at most 2^24 - 1 sequences, 2^30 steps and 2^19 channels", fn);
+        return SNN_ERR_UNSUPPORTED;
+    }
     if (a->seq.lengths && a->seq.offsets) { snn_set_error("%s: lengths and offsets exclude each other", fn); return SNN_ERR_ARG; }
     return SNN_OK;
 }
@@ -361,7 +365,7 @@ template <typename T, int V, int W> int launch(const snn_conv_args* a, int what,
     p.items = (int64_t)a->seq.n_seq * p.nc;
     if (what == BWD) p.slots = bwd_slots(a, V);
     const int64_t blocks = ((what == BWD ? (int64_t)p.slots : p.items) * p.cv + 255) / 256;
-    if (blocks > 0x7fffffff) { snn_set_error("convolution: %lld workgroups", (long long)blocks); return SNN_ERR_UNSUPPORTED; }
+    if (blocks > SEQ_MAX_BLOCKS) { snn_set_error("convolution: %lld workgroups", (long long)blocks); return SNN_ERR_UNSUPPORTED; }
     const dim3 g((unsigned)blocks), t(256);
     if constexpr (V != 4 || sizeof(T) == 4) {
         if (what == FWD) hipLaunchKernelGGL((conv_fwd_kernel<T, V, W>), g, t, 0, s, p);

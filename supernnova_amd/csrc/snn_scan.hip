@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(snn_seq seq, int D, i
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (i0 + i < n_steps) {
-                h = fmaf(e[i], h, v[i]);
+                h = h == 0.0f ? v[i] : fmaf(e[i], h, v[i]);     // the decay over a chunk of growing states may be inf: 0 stays 0
                 q[(int64_t)(reverse ? n_steps - 1 - i0 - i : i0 + i + 1) * per] = h;
             }
         }
@@ -253,6 +253,10 @@ int snn_scan_check(const snn_scan_args* a, const char* fn)
     }
     if (a->dtype < 0 || a->dtype > 2 || a->states < 1 || a->states > 64) {
         snn_set_error("%s: dtype %d / %d states: supported are dtypes 0..2 (SNN_DT_*) and 1..64 states", fn, a->dtype, a->states);
+        return SNN_ERR_UNSUPPORTED;
+    }
+    if (!snn_sizes_fit(a->seq, a->channels)) {
+        snn_set_error("%s: at most 2^24 - 1 sequences, 2^30 steps and 2^19 channels", fn);
         return SNN_ERR_UNSUPPORTED;
     }
     if (a->seq.lengths && a->seq.offsets) { snn_set_error("%s: lengths and offsets exclude each other", fn); return SNN_ERR_ARG; }
@@ -373,7 +377,7 @@ template <typename T, int K, int LN> int step(const snn_scan_args* a, const Scan
 {
     const ScanP<T> p = scan_params<T>(a, g);
     const int64_t blocks = (int64_t)((a->channels + 256 / LN - 1) / (256 / LN)) * a->seq.n_seq;
-    if (blocks > 0x7fffffff) { snn_set_error("snn_scan_step: %lld workgroups", (long long)blocks); return SNN_ERR_UNSUPPORTED; }
+    if (blocks > SEQ_MAX_BLOCKS) { snn_set_error("snn_scan_step: %lld workgroups", (long long)blocks); return SNN_ERR_UNSUPPORTED; }
     hipLaunchKernelGGL((scan_step_kernel<T, K, LN>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     HIP_CHECK(hipGetLastError());
     return SNN_OK;

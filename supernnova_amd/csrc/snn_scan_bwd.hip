@@ -496,8 +496,8 @@ extern "C" int snn_scan_backward(const snn_scan_args* a, void* stream)
     }
     const ScanGrid g = snn_scan_grid(a);
     const int64_t rows = a->seq.offsets ? a->seq.n_rows : (int64_t)a->seq.n_seq * a->seq.max_T;
-    if ((int64_t)a->seq.n_seq * g.nc > 0x7fffffff || (rows * a->groups * 2 * scan_padded(a->states) + 255) / 256 > 0x7fffffff) {
-        snn_set_error("snn_scan_backward: grid too large");
+    if ((int64_t)a->seq.n_seq * g.nc > 0x7fffffff || (rows * a->groups * (scan_padded(a->states) / 2) + 255) / 256 > SEQ_MAX_BLOCKS) {
+        snn_set_error("snn_scan_backward: %lld rows of B and C are too many for one call", (long long)rows);
         return SNN_ERR_UNSUPPORTED;
     }
     const hipStream_t s = (hipStream_t)stream;

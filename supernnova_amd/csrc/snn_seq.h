@@ -16,6 +16,14 @@ template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
+// Sizes a call may have: t + chunk and (taps + 1) * channels stay below 2^31, and no grid has 2^32 threads.
+constexpr int SEQ_MAX_STEPS = 1 << 30, SEQ_MAX_COUNT = (1 << 24) - 1, SEQ_MAX_CHANNELS = 1 << 19;
+constexpr int64_t SEQ_MAX_BLOCKS = (1 << 24) - 1;
+static inline bool snn_sizes_fit(const snn_seq& s, int channels)
+{
+    return s.n_seq <= SEQ_MAX_COUNT && s.max_T <= SEQ_MAX_STEPS && channels <= SEQ_MAX_CHANNELS;
+}
+
 // One view of the batch: element (sequence b, step t, channel d) is at p[t * st + b * sb + d].
 template <typename T> struct View {
     T* p;

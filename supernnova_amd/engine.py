@@ -560,9 +560,6 @@ def _clip(tensors, max_norm, norm_type, grad_scale, out):
     ptrs = array.array("Q", [t.data_ptr() for t in src])
     dst = None
     if out is not None:
-        apart = set(ptrs)
-        if len(apart) != n and len({p for p, k in zip(ptrs, numel) if k}) != sum(map(bool, numel)):
-            raise L.SnnError("a gradient is listed twice")
         if out is src:
             dst = ptrs
         else:
@@ -575,11 +572,6 @@ def _clip(tensors, max_norm, norm_type, grad_scale, out):
                          [(o.shape, o.stride()) for o in out] == [(t.shape, t.stride()) for t in src]):
                 raise L.SnnError("out must match the gradients in elements, strides, type and device")
             dst = array.array("Q", [o.data_ptr() for o in out])
-            if len(set(dst)) != n or not apart.isdisjoint(dst):
-                pairs = [(d, s) for d, s, k in zip(dst, ptrs, numel) if k]
-                to = {d for d, s in pairs}
-                if len(to) != len(pairs) or any(s in to and s != d for d, s in pairs):
-                    raise L.SnnError("out lists a tensor twice, or the place of another gradient")
     lib = L.load()
     dts = array.array("i", dts)
     at = numel.buffer_info()[0]
@@ -600,8 +592,9 @@ def grad_norm(tensors, norm_type=2.0):
 
 def clip_grads(tensors, max_norm, norm_type=2.0, out=None):
     """Multiply every gradient by min(1, max_norm / (norm + 1e-6)), in place, or into `out`, a list of tensors like them
-    (contiguous ones may have another shape: slices of a flat buffer); returns the norm from before as a 0-dim fp32 device tensor.  Gradients that are not finite are not looked for: a norm of
-    inf gives 0 (and NaN where a gradient is inf), a norm of NaN gives NaN, as torch.nn.utils.clip_grad_norm_."""
+    (contiguous ones may have another shape: slices of a flat buffer); returns the norm from before as a 0-dim fp32 device
+    tensor.  Results that overlap each other or another gradient are refused.  Gradients that are not finite are not looked for:
+    a norm of inf gives 0 (and NaN where a gradient is inf), a norm of NaN gives NaN, as torch.nn.utils.clip_grad_norm_."""
     tensors = list(tensors)
     return _clip(tensors, float(max_norm), norm_type, 1.0, tensors if out is None else out)[0]
 
@@ -614,7 +607,7 @@ def clip_coefficient(flat, max_norm, norm_type=2.0, grad_scale=1.0):
 
 def _check_clip(clip):
     _require_cuda(clip, "clip")
-    if clip.numel() != 2:
+    if clip.numel() != 2 or clip.dtype != torch.float32:
         raise L.SnnError("clip must be what clip_coefficient returned")
     return ctypes.c_void_p(clip.data_ptr() + 4)
 

@@ -13,7 +13,7 @@ may be strided (a slice of a wider projection needs no copy):
                `max_len`: a bound on the lengths known to the host (default: the number of rows; a good one saves workspace)
 Rows that belong to no step (behind a sequence's end, outside every sequence, past max_len) are never read, and zero in every
 output.  A sequence of length 0 hands its initial state on.  Lengths and offsets stay on the device (no synchronisation);
-values out of range are cut to the tensors.
+values out of range are cut to the tensors.  Offsets must not decrease: rows that two sequences share have no defined result.
 
 x, delta, z, B, C and what has their shape are float32, bfloat16 or float16, one type per call; parameters, their gradients and
 scan states are float32, sums and states are held in float32, and results are rounded once.  B and C are (.., N) or, with
@@ -308,8 +308,8 @@ def selective_scan_backward(x, delta, A, B, C, dy, tape, D=None, z=None, delta_b
     dy, Dm, sizes = _unit(dy), bt.D, (bt.B, bt.D, N)
     vdy, state, dend = bt.view(dy, "dy"), bt.param(initial_state, "initial_state", sizes), bt.param(dfinal_state, "dfinal_state", sizes)
     n_tape, _, need = _scan_sizes(head[5], Dm, N, G, bt.B, bt.T, bt.seq[2], lengths is not None, offsets is not None)
-    if tape.numel() < n_tape:
-        _fail(f"the tape is too small: {tape.numel()} floats, {n_tape} needed (of selective_scan_train over the same inputs)")
+    if tape is None or tape.numel() < n_tape:
+        _fail(f"the tape is too small: {0 if tape is None else tape.numel()} floats, {n_tape} needed (of selective_scan_train over the same inputs)")
     tape_p = bt.param(tape, "tape", tape.shape)
     (dx, vdx), (ddelta, vdd), (dB, vdB), (dC, vdC) = bt.empty(), bt.empty(), bt.empty(shape), bt.empty(shape)
     dz, vdz = bt.empty() if z is not None else (None, _NO_VIEW)

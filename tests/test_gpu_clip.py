@@ -223,3 +223,16 @@ def test_settings_clip_the_training_step():
     # moves it by lr 1e-8 |g| 2^-24 / (|g| + 1e-8)^2 <= lr / 4 2^-24 each; 16 of them, and 4 of a parameter below 1
     assert float(opt.last_grad_norm) > 0.01
     assert float((rnn.flat_parameters() - twin.flat_parameters()).abs().max()) <= (16 * 1e-2 / 4 + 4) * R.EPS32
+
+
+def test_overlapping_slices_are_refused():
+    flat = torch.randn(100, device="cuda")
+    before = flat.clone()
+    with pytest.raises(L.SnnError, match="overlap"):
+        E.clip_grads([flat[:60], flat[50:]], 0.5)
+    with pytest.raises(L.SnnError, match="overlap"):
+        E.clip_grads([flat[:50]], 0.5, out=[flat[1:51]])
+    assert torch.equal(flat, before)
+    E.clip_grads([flat[50:], flat[:50]], 0.5)                   # neighbours, in any order
+    assert abs(float(flat.double().norm()) - 0.5) <= 2e-6
+    assert float(E.grad_norm([flat, flat])) > float(E.grad_norm([flat]))            # reading twice is no write

@@ -559,3 +559,27 @@ def test_long_sequences_and_many_of_them():
     g1 = ssm.selective_scan_backward(*part, torch.ones_like(y1), tape1)
     assert torch.equal(y[:, 69990:], y1) and torch.equal(gr.dx[:, 69990:], g1.dx) and torch.equal(gr.dB[:, 69990:], g1.dB)
     assert torch.equal(ssm.causal_conv_forward(many[0], rnd(8, 4))[0].isfinite().all(), torch.tensor(True, device="cuda"))
+
+
+def test_growing_states_that_are_still_zero_stay_zero():
+    """Decays above one whose product over a chunk of the time axis overflows, before the first input and behind the last
+    gradient that is not zero: 0 times that product is 0, as step by step."""
+    g = torch.Generator().manual_seed(4)
+    T, D, N = 400, 8, 4
+    x, B, C = torch.randn(1, T, D, generator=g), torch.randn(1, T, N, generator=g), torch.randn(1, T, N, generator=g)
+    delta = torch.full((1, T, D), 2.0)
+    delta[:, 350:] = -1.0
+    x[:, :350] = 0
+    dy = torch.randn(1, T, D, generator=g)
+    dy[:, 20:] = 0
+    A = torch.ones(D, N)
+    x, delta, A, B, C, dy = (t.cuda() for t in (x, delta, A, B, C, dy))
+    y, end, tape = ssm.selective_scan_train(x, delta, A, B, C, delta_softplus=False, want_final_state=True, time_major=False)
+    gr = ssm.selective_scan_backward(x, delta, A, B, C, dy, tape, delta_softplus=False, time_major=False)
+    wide = lambda t: np.repeat(_np(t[0])[:, None], D, axis=1)                                     # noqa: E731
+    args, kw = (_np(x[0]), _np(delta[0]), _np(A), wide(B), wide(C)), dict(sp=False, dy=_np(dy[0]))
+    ref, mag = R.scan(*args, **kw), R.scan(*args, mag=True, **kw)
+    R.close(_np(y[0]), ref["y"], mag["y"], 16 * T + 32)
+    R.close(_np(end[0]), ref["end"], mag["end"], 16 * T + 32)
+    R.close(_np(gr.dx[0]), ref["dx"], mag["dx"], 32 * T + 64)
+    R.close(_np(gr.dA), ref["dA"], mag["dA"], 33 * T + 64)

@@ -160,3 +160,35 @@ def test_autograd_is_refused_while_capturing(monkeypatch):
         ssm.causal_conv(x, torch.zeros(4, 3))
     with pytest.raises(L.SnnError, match="captured"):
         ssm.selective_scan(x, x, torch.zeros(4, 5), torch.zeros(3, 2, 5), torch.zeros(3, 2, 5))
+
+
+def test_c_abi_refuses_sizes_beyond_the_grids():
+    lib = L.load()
+    for n, t, d in ((1 << 24, 4, 8), (1, (1 << 30) + 1, 8), (1, 4, (1 << 19) + 1)):
+        a = L.SnnConvArgs(seq=L.SnnSeq(n, t, 0, None, None), channels=d, width=4)
+        assert lib.snn_conv_forward(ctypes.byref(a), None) == -2 and "at most" in _err()
+        assert lib.snn_conv_workspace_bytes(ctypes.byref(a)) == -2
+        b = L.SnnScanArgs(seq=L.SnnSeq(n, t, 0, None, None), channels=d, groups=1, states=16)
+        assert lib.snn_scan_forward(ctypes.byref(b), None) == -2 and "at most" in _err()
+        assert lib.snn_scan_tape_floats(ctypes.byref(b)) == -2
+    v = L.SnnView(4096, 0, 3)                  # one step of more sequences x channels than a grid of single channels holds
+    a = L.SnnConvArgs(seq=L.SnnSeq((1 << 24) - 1, 1, 0, None, None), channels=257, width=2, x=v, y=v, weight=4096, state_in=4096, state_out=4096)
+    assert lib.snn_conv_step(ctypes.byref(a), None) == -2 and "workgroups" in _err()
+
+
+def test_c_abi_clip_refuses_overlaps():
+    """Addresses only: nothing is launched."""
+    lib = L.load()
+
+    def clip(src, dst, numel, dtype):
+        n = len(src)
+        arr = lambda t, v: (t * n)(*v)                                                            # noqa: E731
+        return lib.snn_clip_grads(n, arr(ctypes.c_void_p, src), arr(ctypes.c_void_p, dst), arr(ctypes.c_int64, numel), arr(ctypes.c_int32, dtype),
+                                  2, 1.0, 1.0, 4096, 4096, 64, None)
+    a, b = 1 << 20, 2 << 20
+    assert clip([a, a + 16], [a, a + 16], [5, 5], [0, 0]) == -1 and "twice" in _err()           # 20 bytes at a
+    assert clip([a, a + 8], [a, a + 8], [5, 5], [1, 1]) == -1 and "twice" in _err()             # 10 bytes at a
+    assert clip([a, b], [b, a], [5, 5], [0, 0]) == -1 and "another gradient" in _err()
+    assert clip([a, b], [a, a + 40], [20, 5], [0, 0]) == -1 and "twice" in _err()               # inside a longer one
+    assert clip([a], [a + 4], [5], [0]) == -1 and "in part" in _err()
+    assert clip([a, b], [b + 64, b + 20 - 4], [5, 5], [0, 0]) == -1 and "in part" in _err()
