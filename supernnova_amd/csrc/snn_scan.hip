@@ -9,7 +9,7 @@
 // where channels x sequences do not fill the chip, the time axis is cut into chunks that run side by side.  Then
 // scan_state_kernel finds every chunk's last state from a zero start (and the sum of its steps: the decay over the
 // whole chunk is exp(A sum s)), scan_combine_kernel runs over the chunks, and scan_fwd_kernel starts each chunk from its
-// true state: 1.6 times the time of a single pass that filled the chip, over `nc` times the lanes.
+// true state: 1.7 times the time of a single pass that filled the chip, over `nc` times the lanes.
 #include <algorithm>
 #include "snn_host.h"
 #include "snn_scan.h"
@@ -269,10 +269,12 @@ int snn_scan_check(const snn_scan_args* a, const char* fn)
 }
 
 // Chunks of the time axis.  One chunk (no arithmetic twice) once the workgroups of a single pass give every SIMD two waves
-// (512 workgroups); below that, as many chunks as bring the grid to 2048 workgroups, none shorter than 64 steps.  More, shorter
-// chunks even out ragged lengths and the grid's last round, but scan_combine_kernel walks over them one by one.  State pass +
-// combination + scan in us, grids of 1024 / 2048 / 4096 workgroups: one prompt of 8191 x 4096 bf16 124 + 5 + 194 / 114 + 8 + 185 /
-// 115 + 13 + 183; seven ragged prompts of up to 1501 x 1536 fp16 52 + 5 + 78 / 44 + 5 + 60 / 36 + 8 + 55.
+// (512 workgroups): whole calls of 1024 steps x 4096 channels bf16, split / not, 138 / 148 us at 256 workgroups, 185 / 194 at
+// 384, 234 / 195 at 512.  Below that, as many chunks as bring the grid to 2048 workgroups, none shorter than 64 steps; 4096 for
+// sequences of different lengths, whose empty chunks leave the chip half full otherwise.  scan_combine_kernel walks over the chunks
+// one by one.  State pass + combination + scan in us, grids of 1024 / 2048 / 4096 / 8192 workgroups: one prompt of 8191 x 4096
+// bf16 124 + 5 + 194 / 111 + 7 + 171 / 112 + 12 + 174 / 106 + 19 + 177; seven ragged prompts of up to 1501 x 1536 fp16
+// 52 + 5 + 78 / 43 + 5 + 59 / 37 + 7 + 54 / 35 + 11 + 52.
 ScanGrid snn_scan_grid(const snn_scan_args* a)
 {
     ScanGrid g;
@@ -282,14 +284,16 @@ ScanGrid snn_scan_grid(const snn_scan_args* a)
     g.blocks_c = g.cbg * a->groups;
     const int64_t blocks = (int64_t)g.blocks_c * a->seq.n_seq;
     int64_t nc = 1;
-    if (blocks < 512) nc = std::min<int64_t>((2048 + blocks - 1) / blocks, (a->seq.max_T + 63) / 64);
+    const int64_t target = a->seq.lengths || a->seq.offsets ? 4096 : 2048;
+    if (blocks < 512) nc = std::min<int64_t>((target + blocks - 1) / blocks, (a->seq.max_T + 63) / 64);
     g.tc = (int)(((a->seq.max_T + nc - 1) / nc + SCAN_SEG - 1) / SCAN_SEG * SCAN_SEG);
     g.nc = (a->seq.max_T + g.tc - 1) / g.tc;
     return g;
 }
 
 // Longest first pays where the grid runs in a few rounds (512 workgroups and more, one chunk a sequence) over sequences of different
-// lengths; beyond 4096 sequences the rounds are many and even out, and the ranks would cost more than they give.
+// lengths: training of 512 x 300 x 256 fp32 504 -> 410 us, the ranks' 2 x 5 us included.  Beyond 4096 sequences the rounds are many
+// and even out, and the ranks, whose time goes with the square of the sequences, would cost more than they give.
 bool snn_scan_ordered(const snn_scan_args* a, const ScanGrid& g)
 {
     return (a->seq.lengths || a->seq.offsets) && (int64_t)g.blocks_c * a->seq.n_seq >= 512 && a->seq.n_seq > 1 && a->seq.n_seq <= 4096;
