@@ -7,7 +7,10 @@
 // and a captured call keeps its own table.  Work is cut into pieces of CLIP_PIECE elements; a workgroup finds its tensor in the
 // table and leaves one fp64 partial sum per piece (squares of fp32 gradients overflow fp32 from 2e19 on).  Up to
 // CLIP_DIRECT pieces -- this framework's own models -- every workgroup of the second pass adds the partial sums itself; above, a
-// single workgroup does it in between.
+// single workgroup does it in between: a call with limits of 0 / 1024 / 8192 at 30 pieces 27.6 / 24.4 / 25.0, at 250 27.5 / 24.3 /
+// 24.6, at 1000 35.6 / 34.6 / 34.6, at 4000 143.5 / 143.5 / 146.3 us.
+// 405 M bf16 elements in 168 tensors: first pass 104 + 57, sum 6, second pass 145 + 132 us: 2.4 GB at 5.5 TB/s (a large copy: 4.7;
+// the end of the first pass is still in the last-level cache when the second begins there).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <algorithm>

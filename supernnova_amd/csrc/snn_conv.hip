@@ -7,7 +7,8 @@
 // ~2W + 10 operations for two (backward: three) elements moved: the memory bounds it.  A thread owns V neighbouring channels
 // (16 bytes of a row, 8 .. 16 in the backward) and walks a chunk of the time axis with the window in registers, so a row is
 // read once but for the W - 1 rows in front of a chunk.  Threads are numbered (chunk of a sequence, channel vector), so
-// narrow layers fill their waves too.
+// narrow layers fill their waves too.  Measured: forward of 8192 x 4096 bf16 27.5 us = 4.9 TB/s (a large copy: 4.7); training of
+// 2048 x 300 x 256 fp32, half of whose rows are padding, forward 197, backward 307, sums 10 us for 2.2 GB.
 #include "snn_seq.h"
 #include "snn_host.h"
 #include <algorithm>

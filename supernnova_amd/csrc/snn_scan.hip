@@ -10,6 +10,8 @@
 // scan_state_kernel finds every chunk's last state from a zero start (and the sum of its steps: the decay over the
 // whole chunk is exp(A sum s)), scan_combine_kernel runs over the chunks, and scan_fwd_kernel starts each chunk from its
 // true state: 1.7 times the time of a single pass that filled the chip, over `nc` times the lanes.
+// One prompt of 8191 x 4096 bf16, 16 states: 111 + 7 + 171 us, 22 and 33 vector instructions a lane's step of four states where the
+// formula takes 16 and 20, the vector unit busy 0.96 and 0.89 of the time.  16384 sequences of up to 40 x 64 fp32: 120 us.
 #include <algorithm>
 #include "snn_host.h"
 #include "snn_scan.h"
@@ -201,7 +203,8 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(snn_seq seq, int D, i
 }
 
 // One step: 8 bytes of fp32 state per (channel, state) in and out, all else is a percent of that: the memory bounds it.
-// The same lanes; a wave reads its neighbouring channels' states as one block, 16 bytes a lane, of R sequences at once.
+// The same lanes; a wave reads its neighbouring channels' states as one block, 16 bytes a lane.  256 sequences x 4096 channels x 16
+// states: 31 us with the state in the last-level cache, 40 us a call at 151 MB; two or four sequences a thread: 41 and 42.
 template <typename T, int K, int LN> __global__ void __launch_bounds__(256) scan_step_kernel(const ScanP<T> p)
 {
     constexpr int CH = 256 / LN;

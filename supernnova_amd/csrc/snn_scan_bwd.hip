@@ -11,6 +11,11 @@
 // halves the number of live values while it adds, then DPP rotations, then LDS over the four waves, then -- layers wider than
 // one workgroup's channels -- fp32 partial rows per channel block, added in order by scan_bc_sum_kernel.  Parameter gradients stay in registers over
 // all chunks a workgroup takes and are summed in fp64, in order, by scan_param_sum_kernel.  No atomics.
+//
+// The vector unit bounds it: 108 instructions a lane's step of four states (27 to recompute, 56 for the adjoint, of which the
+// channel sums take 22 issue slots; the rest per segment), at two waves a SIMD (256 registers; three or four waves spill: 880
+// and 1254 us instead of 297).  4 x 2048 x 2048 bf16 of 16 states: adjoint pass 63, combination 6, this kernel 301, sums 8 + 17 us;
+// 512 x 300 x 256 fp32: 323 us, sums 6 + 22 us.
 #include <algorithm>
 #include "snn_host.h"
 #include "snn_scan.h"
