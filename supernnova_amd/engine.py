@@ -553,11 +553,11 @@ def _clip(tensors, max_norm, norm_type, grad_scale, out):
         dts = [_DTYPES[types[0]]] * n if types.count(types[0]) == n else [_DTYPES[d] for d in types]
     except KeyError as e:
         raise L.SnnError(f"gradients of type {e.args[0]}: supported are float32, bfloat16 and float16") from None
-    whole = all([t.is_contiguous() for t in src])
-    if [t.get_device() for t in src].count(dev.index) != n or not (whole or all(_dense(t) for t in src)):
+    T = torch.Tensor
+    whole = all(map(T.is_contiguous, src))
+    if list(map(T.get_device, src)).count(dev.index) != n or not (whole or all(map(_dense, src))):
         raise L.SnnError("gradients must be dense tensors (no gaps, no repeated elements) on one device")
-    numel = array.array("q", [t.numel() for t in src])
-    ptrs = array.array("Q", [t.data_ptr() for t in src])
+    numel, ptrs = array.array("q", list(map(T.numel, src))), array.array("Q", list(map(T.data_ptr, src)))
     dst = None
     if out is not None:
         if out is src:
@@ -566,22 +566,22 @@ def _clip(tensors, max_norm, norm_type, grad_scale, out):
             out = list(out)
             if len(out) != n:
                 raise L.SnnError(f"out has {len(out)} tensors for {n} gradients")
-            if [o.dtype for o in out] != types or array.array("q", [o.numel() for o in out]) != numel or \
-                    [o.get_device() for o in out].count(dev.index) != n or \
-                    not (whole and all([o.is_contiguous() for o in out]) or
+            if [o.dtype for o in out] != types or array.array("q", list(map(T.numel, out))) != numel or \
+                    list(map(T.get_device, out)).count(dev.index) != n or \
+                    not (whole and all(map(T.is_contiguous, out)) or
                          [(o.shape, o.stride()) for o in out] == [(t.shape, t.stride()) for t in src]):
                 raise L.SnnError("out must match the gradients in elements, strides, type and device")
-            dst = array.array("Q", [o.data_ptr() for o in out])
+            dst = array.array("Q", list(map(T.data_ptr, out)))
     lib = L.load()
     dts = array.array("i", dts)
     at = numel.buffer_info()[0]
     doubles = L.check(lib.snn_clip_scratch_doubles(n, at), "snn_clip_scratch_doubles")
-    buf = torch.empty(1 + doubles, dtype=torch.float64, device=dev)
-    p = buf.data_ptr()
+    res, scratch = torch.empty(2, dtype=torch.float32, device=dev), torch.empty(doubles, dtype=torch.float64, device=dev)
     with _on_device(dev):
         L.check(lib.snn_clip_grads(n, ptrs.buffer_info()[0], None if dst is None else dst.buffer_info()[0], at, dts.buffer_info()[0],
-                                   code, max_norm, grad_scale, p, p + 8, doubles, _stream()), "snn_clip_grads")
-    return buf[:1].view(torch.float32)
+                                   code, max_norm, grad_scale, res.data_ptr(), scratch.data_ptr(), doubles,
+                                   torch._C._cuda_getCurrentRawStream(dev.index)), "snn_clip_grads")
+    return res
 
 
 def grad_norm(tensors, norm_type=2.0):

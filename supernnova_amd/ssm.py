@@ -79,7 +79,7 @@ class _Batch:
         if x.dtype not in E._DTYPES:
             _fail(f"x must be float32, bfloat16 or float16, got {x.dtype}")
         shape = x.shape
-        self.dtype, self.device, self.index, self.shape = x.dtype, x.device, x.get_device(), shape
+        self.x, self.dtype, self.device, self.index, self.shape = x, x.dtype, x.device, x.get_device(), shape
         lengths_p = offsets_p = rows = 0
         if offsets is not None:
             if len(shape) != 2:
@@ -123,7 +123,7 @@ class _Batch:
 
     def empty(self, shape=None):
         """A contiguous result of x's (or the given) shape, and its snn_view."""
-        t = torch.empty(self.shape if shape is None else shape, dtype=self.dtype, device=self.device)
+        t = self.x.new_empty(*(self.shape if shape is None else shape))       # two thirds of the time torch.empty takes
         st = t.stride()
         return t, (t.data_ptr(), st[self.t_dim], 0 if self.n_dim is None else st[self.n_dim])
 
@@ -134,9 +134,6 @@ class _Batch:
         if t.dtype != dtype or t.get_device() != self.index or t.shape != shape or not t.is_contiguous():
             _fail(f"{name} must be contiguous {dtype} {shape} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         return t.data_ptr()
-
-    def floats(self, *shape):
-        return torch.empty(shape, dtype=torch.float32, device=self.device)
 
     def launch(self, fn, what, args):
         if self.index == torch.cuda.current_device():
@@ -153,7 +150,7 @@ class _Step(_Batch):
         _on_gpu(x)
         if x.dtype not in E._DTYPES or x.dim() != 2 or x.numel() < 1:
             _fail(f"x must be a non-empty (sequences, channels) tensor of float32, bfloat16 or float16, got {x.dtype} {tuple(x.shape)}")
-        self.dtype, self.device, self.index, self.shape = x.dtype, x.device, x.get_device(), x.shape
+        self.x, self.dtype, self.device, self.index, self.shape = x, x.dtype, x.device, x.get_device(), x.shape
         self.B, self.D = self.shape
         self.T, self.t_dim, self.n_dim, self.lead = 1, 0, 0, self.shape[:1]
         self.seq = (self.B, 1, 0, 0, 0)
@@ -192,7 +189,7 @@ def causal_conv_forward(x, weight, bias=None, *, activation="silu", lengths=None
     W, head, par = _conv_head(bt, weight, bias, activation)
     vx, state = bt.view(x, "x"), bt.param(initial_state, "initial_state", (bt.B, W - 1, bt.D), bt.dtype)
     y, vy = bt.empty()
-    end = torch.empty((bt.B, W - 1, bt.D), dtype=bt.dtype, device=bt.device) if want_final_state else None
+    end = x.new_empty(bt.B, W - 1, bt.D) if want_final_state else None
     bt.launch(L.load().snn_conv_forward, "snn_conv_forward",
               _CONV.pack(*head, *vx, *vy, *_NO_VIEW, *_NO_VIEW, *par, state, 0 if end is None else end.data_ptr(), 0, 0, 0, 0, 0, 0))
     return y, end
@@ -208,13 +205,13 @@ def causal_conv_backward(x, weight, bias, dy, *, dfinal_state=None, activation="
     vx, vdy, state = bt.view(x, "x"), bt.view(dy, "dy"), bt.param(initial_state, "initial_state", shape, bt.dtype)
     dend = bt.param(dfinal_state, "dfinal_state", shape, bt.dtype)
     dx, vdx = bt.empty()
-    dweight, dbias = bt.floats(bt.D, W), bt.floats(bt.D) if bias is not None else None
+    dweight, dbias = weight.new_empty(bt.D, W), weight.new_empty(bt.D) if bias is not None else None
     dstate = torch.empty_like(initial_state) if initial_state is not None else None
     args = (*head, *vx, *_NO_VIEW, *vdy, *vdx, *par, state, 0, dend, 0 if dstate is None else dstate.data_ptr(), dweight.data_ptr(),
             0 if dbias is None else dbias.data_ptr())
     lib = L.load()
     need = L.check(lib.snn_conv_workspace_bytes(_CONV.pack(*args, 0, 0)), "snn_conv_workspace_bytes")
-    ws = bt.floats(need // 4)
+    ws = weight.new_empty(need // 4)
     bt.launch(lib.snn_conv_backward, "snn_conv_backward", _CONV.pack(*args, ws.data_ptr(), need))
     return ConvGrads(dx, dweight, dbias, dstate)
 
@@ -274,9 +271,9 @@ def _scan_forward(x, delta, A, B, C, D, z, delta_bias, delta_softplus, lengths, 
     head, G, N, _ = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, vy)
     state = bt.param(initial_state, "initial_state", (bt.B, bt.D, N))
     n_tape, need, _ = _scan_sizes(head[5], bt.D, N, G, bt.B, bt.T, bt.seq[2], lengths is not None, offsets is not None)
-    end = bt.floats(bt.B, bt.D, N) if want_final_state else None
-    tape = bt.floats(n_tape) if want_tape else None
-    ws = bt.floats(need // 4) if need else None
+    end = A.new_empty(bt.B, bt.D, N) if want_final_state else None
+    tape = A.new_empty(n_tape) if want_tape else None
+    ws = A.new_empty(need // 4) if need else None
     bt.launch(L.load().snn_scan_forward, "snn_scan_forward",
               _SCAN.pack(*head, state, 0 if end is None else end.data_ptr(), 0 if tape is None else tape.data_ptr(), n_tape if want_tape else 0,
                          *_NO_GRADS, 0 if ws is None else ws.data_ptr(), need))
@@ -313,10 +310,10 @@ def selective_scan_backward(x, delta, A, B, C, dy, tape, D=None, z=None, delta_b
     tape_p = bt.param(tape, "tape", tape.shape)
     (dx, vdx), (ddelta, vdd), (dB, vdB), (dC, vdC) = bt.empty(), bt.empty(), bt.empty(shape), bt.empty(shape)
     dz, vdz = bt.empty() if z is not None else (None, _NO_VIEW)
-    dA, dD = bt.floats(Dm, N), bt.floats(Dm) if D is not None else None
-    dbias = bt.floats(Dm) if delta_bias is not None else None
+    dA, dD = A.new_empty(Dm, N), A.new_empty(Dm) if D is not None else None
+    dbias = A.new_empty(Dm) if delta_bias is not None else None
     dstate = torch.empty_like(initial_state) if initial_state is not None else None
-    ws = bt.floats(need // 4)
+    ws = A.new_empty(need // 4)
     bt.launch(L.load().snn_scan_backward, "snn_scan_backward",
               _SCAN.pack(*head, state, 0, tape_p, n_tape, *vdy, *vdx, *vdd, *vdz, *vdB, *vdC, dend, dA.data_ptr(), 0 if dD is None else dD.data_ptr(),
                          0 if dbias is None else dbias.data_ptr(), 0 if dstate is None else dstate.data_ptr(), ws.data_ptr(), need))
