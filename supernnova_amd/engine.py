@@ -12,6 +12,7 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as _ad
 
 from . import _lib as L
 
@@ -520,6 +521,13 @@ def ce_loss_grad(logits, target, grad_scale=None):
     return buf[0], dlogits
 
 
+def _no_tangents(*tensors):
+    """Inside a level of forward-mode differentiation: a dual tensor does not require grad, and its tangent would be lost here."""
+    for t in tensors:
+        if t is not None and _ad.unpack_dual(t).tangent is not None:
+            raise L.SnnError("no forward-mode differentiation: a tensor with a tangent was given")
+
+
 _DTYPES = {torch.float32: L.SNN_DT_F32, torch.bfloat16: L.SNN_DT_BF16, torch.float16: L.SNN_DT_F16}
 _NORM_TYPES = {1.0: 1, 2.0: 2, math.inf: 0}
 
@@ -544,6 +552,10 @@ def _clip(tensors, max_norm, norm_type, grad_scale, out):
         raise L.SnnError(f"norm_type {norm_type!r}: supported are 1, 2 and inf")
     if not src:
         raise L.SnnError("no gradients")
+    if torch._C._get_tracing_state() is not None:
+        raise L.SnnError("gradient norms and clipping cannot be traced: the launches are not torch operations")
+    if _ad._current_level >= 0:
+        _no_tangents(*src)
     dev = src[0].device
     if dev.type != "cuda":
         raise L.SnnError("gradients must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")

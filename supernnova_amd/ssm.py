@@ -22,7 +22,8 @@ groups of channels that share them, (.., G, N).  States: convolution (B, W - 1, 
 Two levels, as engine.py / modules.py: `*_forward`, `*_train`, `*_backward`, `*_step` launch kernels on the current stream and can
 be captured into a graph; `causal_conv` and `selective_scan` are their differentiable forms.  The latter refuse to record or run
 a backward pass while a stream is being captured (autograd would accumulate on the streams of whatever graph the leaves were
-in before): capture the explicit pair.  The step functions write the state in place unless given `new_state`.
+in before): capture the explicit pair.  The step functions write the state in place unless given `new_state`.  Forward-mode differentiation and
+torch.jit.trace, which would lose tangents and launches without a word, are refused.
 """
 import ctypes
 import functools
@@ -30,6 +31,7 @@ import struct
 from typing import NamedTuple, Optional
 
 import torch
+import torch.autograd.forward_ad as _ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -71,6 +73,12 @@ def _on_gpu(x):
         _fail("x must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")
 
 
+def _not_traced(size):
+    """torch.jit.trace hands out sizes as tensors; it would record the allocation of the results and nothing that fills them."""
+    if type(size) is not int:
+        _fail("supernnova_amd.ssm cannot be traced: the launches are not torch operations")
+
+
 class _Batch:
     """The layout of one call: sequences, steps, and the strides of a tensor's step and sequence dimensions."""
 
@@ -79,6 +87,7 @@ class _Batch:
         if x.dtype not in E._DTYPES:
             _fail(f"x must be float32, bfloat16 or float16, got {x.dtype}")
         shape = x.shape
+        _not_traced(shape[-1] if len(shape) else 0)
         self.x, self.dtype, self.device, self.index, self.shape = x, x.dtype, x.device, x.get_device(), shape
         lengths_p = offsets_p = rows = 0
         if offsets is not None:
@@ -148,6 +157,7 @@ class _Step(_Batch):
 
     def __init__(self, x):
         _on_gpu(x)
+        _not_traced(x.shape[-1] if x.dim() else 0)
         if x.dtype not in E._DTYPES or x.dim() != 2 or x.numel() < 1:
             _fail(f"x must be a non-empty (sequences, channels) tensor of float32, bfloat16 or float16, got {x.dtype} {tuple(x.shape)}")
         self.x, self.dtype, self.device, self.index, self.shape = x, x.dtype, x.device, x.get_device(), x.shape
@@ -185,6 +195,8 @@ def causal_conv_forward(x, weight, bias=None, *, activation="silu", lengths=None
     """Depthwise causal convolution of a batch of sequences: weight (D, W) with weight[:, -1] on the current step, bias (D,) or
     None, activation "silu" or None.  Returns (y like x, final state (B, W - 1, D) or None); the final state is what
     causal_conv_step and a later call's initial_state go on from."""
+    if _ad._current_level >= 0:
+        E._no_tangents(x, weight, bias, initial_state)
     bt = _Batch(x, lengths, offsets, max_len, time_major)
     W, head, par = _conv_head(bt, weight, bias, activation)
     vx, state = bt.view(x, "x"), bt.param(initial_state, "initial_state", (bt.B, W - 1, bt.D), bt.dtype)
@@ -199,6 +211,8 @@ def causal_conv_backward(x, weight, bias, dy, *, dfinal_state=None, activation="
                          initial_state=None, time_major=True):
     """Gradients of causal_conv_forward's result from dy = dloss/dy and, if the final state was used, dfinal_state.  Sums over
     sequences and steps are taken in an order that depends on the sizes alone."""
+    if _ad._current_level >= 0:
+        E._no_tangents(x, weight, bias, dy, dfinal_state, initial_state)
     bt = _Batch(x, lengths, offsets, max_len, time_major)
     W, head, par = _conv_head(bt, weight, bias, activation)
     dy, shape = _unit(dy), (bt.B, W - 1, bt.D)
@@ -219,6 +233,8 @@ def causal_conv_backward(x, weight, bias, dy, *, dfinal_state=None, activation="
 def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_state=None):
     """The convolution's output for one new input x (B, D) of every sequence; `state` (B, W - 1, D) holds the inputs before
     it and is moved on in place, or left as it is and its successor written to `new_state`."""
+    if _ad._current_level >= 0:
+        E._no_tangents(x, state, weight, bias, new_state)
     bt = _Step(x)
     if state is None:
         _fail("causal_conv_step needs the state")
@@ -266,6 +282,8 @@ _NO_GRADS = (*(6 * _NO_VIEW), 0, 0, 0, 0, 0)
 
 def _scan_forward(x, delta, A, B, C, D, z, delta_bias, delta_softplus, lengths, offsets, max_len, initial_state, want_final_state,
                   time_major, want_tape):
+    if _ad._current_level >= 0:
+        E._no_tangents(x, delta, A, B, C, D, z, delta_bias, initial_state)
     bt = _Batch(x, lengths, offsets, max_len, time_major)
     y, vy = bt.empty()
     head, G, N, _ = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, vy)
@@ -300,6 +318,8 @@ def selective_scan_backward(x, delta, A, B, C, dy, tape, D=None, z=None, delta_b
                             lengths=None, offsets=None, max_len=None, initial_state=None, time_major=True):
     """Gradients from dy = dloss/dy and, if the final state was used, dfinal_state, with the tape of selective_scan_train over the
     same inputs.  Every sum is taken in an order that depends on the sizes alone."""
+    if _ad._current_level >= 0:
+        E._no_tangents(x, delta, A, B, C, dy, tape, D, z, delta_bias, dfinal_state, initial_state)
     bt = _Batch(x, lengths, offsets, max_len, time_major)
     head, G, N, shape = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, _NO_VIEW)
     dy, Dm, sizes = _unit(dy), bt.D, (bt.B, bt.D, N)
@@ -323,6 +343,8 @@ def selective_scan_backward(x, delta, A, B, C, dy, tape, D=None, z=None, delta_b
 def selective_scan_step(x, state, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_softplus=True, new_state=None):
     """One step of every sequence: x, delta, z (B, D), B, C (B, [G,] N); `state` (B, D, N) float32 is moved on in place, or left as
     it is and its successor written to `new_state`.  Returns y (B, D)."""
+    if _ad._current_level >= 0:
+        E._no_tangents(x, state, delta, A, B, C, D, z, delta_bias, new_state)
     bt = _Step(x)
     if state is None:
         _fail("selective_scan_step needs the state")
