@@ -593,6 +593,8 @@ def _clip(tensors, max_norm, norm_type, grad_scale, out):
         L.check(lib.snn_clip_grads(n, ptrs.buffer_info()[0], None if dst is None else dst.buffer_info()[0], at, dts.buffer_info()[0],
                                    code, max_norm, grad_scale, res.data_ptr(), scratch.data_ptr(), doubles,
                                    torch._C._cuda_getCurrentRawStream(dev.index)), "snn_clip_grads")
+    if out is not None:
+        torch._C._increment_version(out)        # written through addresses: a backward pass that saved one has to know
     return res
 
 

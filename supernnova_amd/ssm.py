@@ -22,8 +22,9 @@ groups of channels that share them, (.., G, N).  States: convolution (B, W - 1, 
 Two levels, as engine.py / modules.py: `*_forward`, `*_train`, `*_backward`, `*_step` launch kernels on the current stream and can
 be captured into a graph; `causal_conv` and `selective_scan` are their differentiable forms.  The latter refuse to record or run
 a backward pass while a stream is being captured (autograd would accumulate on the streams of whatever graph the leaves were
-in before): capture the explicit pair.  The step functions write the state in place unless given `new_state`.  Forward-mode differentiation and
-torch.jit.trace, which would lose tangents and launches without a word, are refused.
+in before): capture the explicit pair.  Results of the explicit calls carry no history, whatever their arguments require.  The
+step functions write the state in place unless given `new_state`, and refuse to write one that requires grad.  Forward-mode
+differentiation and torch.jit.trace, which would lose tangents and launches without a word, are refused.
 """
 import ctypes
 import functools
@@ -73,10 +74,9 @@ def _on_gpu(x):
         _fail("x must live on a HIP device: supernnova_amd runs only on the GPU (no CPU fallback)")
 
 
-def _not_traced(size):
+def _traced():
     """torch.jit.trace hands out sizes as tensors; it would record the allocation of the results and nothing that fills them."""
-    if type(size) is not int:
-        _fail("supernnova_amd.ssm cannot be traced: the launches are not torch operations")
+    _fail("supernnova_amd.ssm cannot be traced: the launches are not torch operations")
 
 
 class _Batch:
@@ -87,7 +87,8 @@ class _Batch:
         if x.dtype not in E._DTYPES:
             _fail(f"x must be float32, bfloat16 or float16, got {x.dtype}")
         shape = x.shape
-        _not_traced(shape[-1] if len(shape) else 0)
+        if len(shape) and type(shape[0]) is not int:
+            _traced()
         self.x, self.dtype, self.device, self.index, self.shape = x, x.dtype, x.device, x.get_device(), shape
         lengths_p = offsets_p = rows = 0
         if offsets is not None:
@@ -157,21 +158,34 @@ class _Step(_Batch):
 
     def __init__(self, x):
         _on_gpu(x)
-        _not_traced(x.shape[-1] if x.dim() else 0)
-        if x.dtype not in E._DTYPES or x.dim() != 2 or x.numel() < 1:
-            _fail(f"x must be a non-empty (sequences, channels) tensor of float32, bfloat16 or float16, got {x.dtype} {tuple(x.shape)}")
-        self.x, self.dtype, self.device, self.index, self.shape = x, x.dtype, x.device, x.get_device(), x.shape
+        shape = x.shape
+        if len(shape) and type(shape[0]) is not int:
+            _traced()
+        if x.dtype not in E._DTYPES or len(shape) != 2 or x.numel() < 1:
+            _fail(f"x must be a non-empty (sequences, channels) tensor of float32, bfloat16 or float16, got {x.dtype} {tuple(shape)}")
+        self.x, self.dtype, self.device, self.index, self.shape = x, x.dtype, x.device, x.get_device(), shape
         self.B, self.D = self.shape
         self.T, self.t_dim, self.n_dim, self.lead = 1, 0, 0, self.shape[:1]
         self.seq = (self.B, 1, 0, 0, 0)
 
 
-def _apart(state, new_state, address):
-    """new_state's address; the two may be one buffer, but must not overlap in part (other sequences would read what is written)."""
-    gap = abs(address - state.data_ptr())
+# Tells autograd that tensors written through their addresses have other values now: a backward pass that saved one raises instead of
+# reading them.
+_increment_version = torch._C._increment_version
+
+
+def _apart(state, old, new):
+    """The state and what a step writes, at these addresses: the two may be one buffer, but must not overlap in part (other
+    sequences would read what is written)."""
+    gap = abs(new - old)
     if 0 < gap < state.numel() * state.element_size():
         _fail("state and new_state overlap")
-    return address
+
+
+def _written_requires_grad():
+    """Written through its address, a tensor would keep the history of the values before."""
+    if torch.is_grad_enabled():
+        _fail("the state to be written requires grad: the step functions have no gradient (call them under torch.no_grad(), or detach the state)")
 
 
 def _unit(t):
@@ -241,9 +255,16 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_stat
     W, head, par = _conv_head(bt, weight, bias, activation)
     shape = (bt.B, W - 1, bt.D)
     vx, old = bt.view(x, "x"), bt.param(state, "state", shape, bt.dtype)
-    new = old if new_state is None else _apart(state, new_state, bt.param(new_state, "new_state", shape, bt.dtype))
+    if new_state is None:
+        new_state, new = state, old
+    else:
+        new = bt.param(new_state, "new_state", shape, bt.dtype)
+        _apart(state, old, new)
+    if new_state.requires_grad:
+        _written_requires_grad()
     y, vy = bt.empty()
     bt.launch(L.load().snn_conv_step, "snn_conv_step", _CONV.pack(*head, *vx, *vy, *_NO_VIEW, *_NO_VIEW, *par, old, new, 0, 0, 0, 0, 0, 0))
+    _increment_version((new_state,))
     return y
 
 
@@ -351,8 +372,15 @@ def selective_scan_step(x, state, delta, A, B, C, D=None, z=None, delta_bias=Non
     y, vy = bt.empty()
     head, _, N, _ = _scan_head(bt, x, delta, A, B, C, D, z, delta_bias, delta_softplus, vy)
     old = bt.param(state, "state", (bt.B, bt.D, N))
-    new = old if new_state is None else _apart(state, new_state, bt.param(new_state, "new_state", (bt.B, bt.D, N)))
+    if new_state is None:
+        new_state, new = state, old
+    else:
+        new = bt.param(new_state, "new_state", (bt.B, bt.D, N))
+        _apart(state, old, new)
+    if new_state.requires_grad:
+        _written_requires_grad()
     bt.launch(L.load().snn_scan_step, "snn_scan_step", _SCAN.pack(*head, old, new, 0, 0, *_NO_GRADS, 0, 0))
+    _increment_version((new_state,))
     return y
 
 

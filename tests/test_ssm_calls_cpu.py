@@ -68,3 +68,45 @@ def test_tracing_is_refused(host_only):
             pytest.fail(name)
     with pytest.raises(L.SnnError, match="traced"):
         torch.jit.trace(lambda g: E.grad_norm([g]), (torch.ones(3),), check_trace=False)
+
+
+def test_steps_tell_autograd_what_they_wrote(host_only):
+    """A state that a differentiable call has saved and a step then moves on in place: the backward pass must not use it."""
+    w = torch.randn(4, 3)
+    for inference in (False, True):
+        with torch.inference_mode(inference):
+            x, s, h, one = torch.randn(2, 4), torch.randn(2, 2, 4), torch.randn(2, 4, 5), _inputs((2,))
+            ssm.causal_conv_step(x, s, w, new_state=torch.empty_like(s))
+            ssm.selective_scan_step(**one, state=h, new_state=torch.empty_like(h))
+            ssm.causal_conv_step(x, s, w)
+            ssm.selective_scan_step(**one, state=h)
+    x, s, h, one = torch.randn(2, 4), torch.randn(2, 2, 4), torch.randn(2, 4, 5), _inputs((2,))
+    s2, h2 = torch.empty_like(s), torch.empty_like(h)
+    was = [t._version for t in (s, h, s2, h2)]
+    ssm.causal_conv_step(x, s, w, new_state=s2)
+    ssm.selective_scan_step(**one, state=h, new_state=h2)
+    assert [t._version for t in (s, h)] == was[:2] and s2._version > was[2] and h2._version > was[3]
+    y = (torch.ones(4, requires_grad=True) * s).sum()
+    ssm.causal_conv_step(x, s, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    y = (torch.ones(5, requires_grad=True) * h).sum()
+    ssm.selective_scan_step(**one, state=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_steps_refuse_to_write_a_state_with_a_gradient(host_only):
+    """The written state would keep the history of the one before it."""
+    w, x, one = torch.randn(4, 3), torch.randn(2, 4), _inputs((2,))
+    for of in (lambda t: t.requires_grad_(), lambda t: t.requires_grad_() * 2):          # a leaf, and a result
+        s, h = of(torch.randn(2, 2, 4)), of(torch.randn(2, 4, 5))
+        s0, h0 = torch.randn(2, 2, 4), torch.randn(2, 4, 5)
+        for call in (lambda: ssm.causal_conv_step(x, s, w), lambda: ssm.causal_conv_step(x, s0, w, new_state=s),
+                     lambda: ssm.selective_scan_step(**one, state=h), lambda: ssm.selective_scan_step(**one, state=h0, new_state=h)):
+            with pytest.raises(L.SnnError, match="requires grad"):
+                call()
+            with torch.no_grad():
+                call()
+        ssm.causal_conv_step(x, s, w, new_state=s0)                      # reading one is no matter
+        ssm.selective_scan_step(**one, state=h, new_state=h0)
