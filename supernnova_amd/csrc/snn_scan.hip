@@ -166,6 +166,17 @@ __global__ void __launch_bounds__(256) scan_order_kernel(const snn_seq seq, int*
     if (lane == 0) order[rank] = b;
 }
 
+// h 2^p + v, p cut to what takes any h to 0 or inf.  2^p itself would overflow for p >= 128 (the decay over a chunk of growing
+// states) where its product with a small h does not: the whole part of p goes to the exponent of h.
+struct Pow2 { float frac; int whole; };
+__device__ __forceinline__ Pow2 pow2_parts(float p)
+{
+    const float q = p < -1000.0f ? -1000.0f : (p > 1000.0f ? 1000.0f : p);                  // a NaN stays
+    const float w = fminf(fmaxf(floorf(p), -1000.0f), 1000.0f);
+    return Pow2{__builtin_amdgcn_exp2f(q - w), (int)w};
+}
+__device__ __forceinline__ float decayed(float h, const Pow2& e, float v) { return fmaf(e.frac, ldexpf(h, e.whole), v); }
+
 // carry[b][c] from the chunks' local results, over the chunks of a sequence.  Forward: slot c holds chunk c-1's local last
 // state; state entering c = exp(A csum[c-1]) (state entering c-1) + slot c, from the initial state.  Reverse: slot c holds
 // what chunk c+1 sends back from a zero start; entering c = slot c + exp(A csum[c+1]) (entering c+1), from `edge` (or 0) in
@@ -185,17 +196,18 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(snn_seq seq, int D, i
     const int n_steps = used - 1;
     if (reverse && used > 0) q[(int64_t)n_steps * per] = h;
     for (int i0 = 0; i0 < n_steps; i0 += 8) {
-        float v[8], e[8];
+        float v[8];
+        Pow2 e[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int k = i0 + i < n_steps ? i0 + i : n_steps - 1, c = reverse ? n_steps - 1 - k : k + 1;
             v[i] = q[c * per];
-            e[i] = __builtin_amdgcn_exp2f(a2 * cs[(int64_t)(reverse ? c + 1 : c - 1) * D]);
+            e[i] = pow2_parts(a2 * cs[(int64_t)(reverse ? c + 1 : c - 1) * D]);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (i0 + i < n_steps) {
-                h = h == 0.0f ? v[i] : fmaf(e[i], h, v[i]);     // the decay over a chunk of growing states may be inf: 0 stays 0
+                h = decayed(h, e[i], v[i]);
                 q[(int64_t)(reverse ? n_steps - 1 - i0 - i : i0 + i + 1) * per] = h;
             }
         }

@@ -1,12 +1,18 @@
 """The sequence operators and clipping as calls beside autograd, and over batches whose shape the other files leave out; values
 against 64-bit forms (tolerances: tests/ssm_reference.py)."""
+import numpy as np
 import pytest
 import torch
 
+import ssm_reference as R
 from supernnova_amd import engine as E
 from supernnova_amd import ssm
 
 pytestmark = pytest.mark.gpu
+
+
+def _np(t):
+    return None if t is None else t.detach().double().cpu().numpy()
 
 
 def test_a_state_moved_on_in_place_is_not_differentiated_through():
@@ -37,3 +43,37 @@ def test_clipping_tells_autograd_what_it_wrote():
     flat = torch.ones(5, device="cuda")
     E.clip_coefficient(flat, 1.0)
     assert flat._version == 0
+
+
+def test_small_states_that_grow_over_a_chunk():
+    """A chunk of the time axis whose decays multiply to more than fp32 holds, over a state, and an adjoint, small enough that the
+    product is finite: 1e-30 e^96."""
+    g = torch.Generator().manual_seed(7)
+    T, D, N = 400, 8, 4
+    rnd = lambda *s: torch.randn(s, generator=g)                                                  # noqa: E731
+    x, B, C, dy, h0 = rnd(1, T, D), rnd(1, T, N), rnd(1, T, N), rnd(1, T, D), rnd(1, D, N)
+    x[:, :128] *= 1e-30
+    x[:, 128:] = 0
+    dy[:, :192] = 0
+    dy[:, 192:] *= 1e-30
+    h0 *= 1e-30
+    delta = torch.full((1, T, D), -0.1)
+    delta[:, :64] = 0.01
+    delta[:, 128:192] = 1.5                          # 64 steps: e^96
+    A = torch.ones(D, N)
+    x, delta, A, B, C, dy, h0 = (t.cuda() for t in (x, delta, A, B, C, dy, h0))
+    kw = dict(delta_softplus=False, initial_state=h0, time_major=False)
+    y, end, tape = ssm.selective_scan_train(x, delta, A, B, C, want_final_state=True, **kw)
+    gr = ssm.selective_scan_backward(x, delta, A, B, C, dy, tape, **kw)
+    wide = lambda t: np.repeat(_np(t[0])[:, None], D, axis=1)                                     # noqa: E731
+    args, rkw = (_np(x[0]), _np(delta[0]), _np(A), wide(B), wide(C)), dict(sp=False, h0=_np(h0[0]), dy=_np(dy[0]))
+    ref, mag = R.scan(*args, **rkw), R.scan(*args, mag=True, **rkw)
+    assert np.abs(ref["y"]).max() > 1e9
+    k = 16 * T + 32
+    R.close(_np(y[0]), ref["y"], mag["y"], k, what="y")
+    R.close(_np(end[0]), ref["end"], mag["end"], k, what="end")
+    for name, got in (("dx", gr.dx[0]), ("ddelta", gr.ddelta[0]), ("dh0", gr.dinitial_state[0])):
+        R.close(_np(got), ref[name], mag[name], 2 * k, what=name)
+    R.close(_np(gr.dA), ref["dA"], mag["dA"], 2 * k + T, what="dA")
+    for name, got in (("dB", gr.dB[0]), ("dC", gr.dC[0])):
+        R.close(_np(got), ref[name].sum(1), mag[name].sum(1), 2 * k + D, what=name)
