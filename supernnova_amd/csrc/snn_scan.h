@@ -75,6 +75,17 @@ template <int K> __device__ __forceinline__ void store_states(float* p, int n, i
     }
 }
 
+// A in powers of two.  Steps of zero -- those that fill up a sequence's last segment, too -- leave the state as it is, so the
+// product must not be infinite: 0 x inf.  At the lowest finite value every other step still decays to 0.
+template <int K> __device__ __forceinline__ void decay_rates(float (&A)[K])
+{
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        A[k] *= SNN_LOG2E;
+        A[k] = A[k] < -3.402823466e38f ? -3.402823466e38f : A[k];          // a NaN stays
+    }
+}
+
 // Steps j, j + 4, .. of a segment of one tensor for lane j, G of them; p points at step j and moves with the segment.  A whole
 // segment adds multiples of the stride, the same for every lane; the last one of a chunk reads the chunk's last step again
 // instead of steps behind it, and the caller drops what it read there.

@@ -69,8 +69,7 @@ template <typename T, int K, int LN, bool STATE_ONLY, bool GATE> __global__ void
             if (!STATE_ONLY) Ci.p += SEG * p.C.st;
         };
         fetch(t1 - t0);                                 // before anything waits for the loads above: one latency, not two
-#pragma unroll
-        for (int k = 0; k < K; ++k) A2[k] *= SNN_LOG2E;
+        decay_rates<K>(A2);
         int buf = 0;
         for (int t = t0; t < t1; t += SEG, buf ^= 1) {
             Bi.store(sB[buf], tid);
@@ -188,7 +187,8 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(snn_seq seq, int D, i
     if (id >= (int64_t)seq.n_seq * per) return;
     const int b = (int)(id / per), e = (int)(id - b * per), d = e / NP, n = e - d * NP;
     const int len = seq_range(seq, b).len, used = (len + tc - 1) / tc;
-    const float a2 = n < N ? A[(int64_t)d * N + n] * SNN_LOG2E : 0.0f;
+    float a2[1] = {n < N ? A[(int64_t)d * N + n] : 0.0f};
+    decay_rates<1>(a2);
     float h = edge && n < N ? edge[((int64_t)b * D + d) * N + n] : 0.0f;
     float* q = carry + (int64_t)b * nc * per + e;
     const float* cs = csum + (int64_t)b * nc * D + d;
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) scan_combine_kernel(snn_seq seq, int D, i
         for (int i = 0; i < 8; ++i) {
             const int k = i0 + i < n_steps ? i0 + i : n_steps - 1, c = reverse ? n_steps - 1 - k : k + 1;
             v[i] = q[c * per];
-            e[i] = pow2_parts(a2 * cs[(int64_t)(reverse ? c + 1 : c - 1) * D]);
+            e[i] = pow2_parts(a2[0] * cs[(int64_t)(reverse ? c + 1 : c - 1) * D]);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -235,13 +235,14 @@ template <typename T, int K, int LN> __global__ void __launch_bounds__(256) scan
         Cv[k] = p.C.p[b * p.C.sb + g * p.C_sg + m];
     }
     load_states<K>(p.A + (int64_t)d * p.N, n, p.N, p.vec, A2);
+    decay_rates<K>(A2);
     const float v = delta + (p.dbias ? p.dbias[d] : 0.0f), skip = p.skip ? p.skip[d] : 0.0f;
     const float s = p.softplus ? softplus_f32(v, nullptr) : v, u = s * x;
     float y = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const bool in = n + k < p.N;
-        h[k] = fmaf(__builtin_amdgcn_exp2f(s * (A2[k] * SNN_LOG2E)), h[k], in ? u * to_f32(Bv[k]) : 0.0f);
+        h[k] = fmaf(__builtin_amdgcn_exp2f(s * A2[k]), h[k], in ? u * to_f32(Bv[k]) : 0.0f);
         y = in ? fmaf(h[k], to_f32(Cv[k]), y) : y;
     }
     y = quad_sum(y);

@@ -93,11 +93,9 @@ template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds_
         Ci.p -= SEG * p.C.st;
     };
     fetch(t1 - tl);
+    decay_rates<K>(A2);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        A2[k] *= SNN_LOG2E;
-        w[k] = 0.0f;
-    }
+    for (int k = 0; k < K; ++k) w[k] = 0.0f;
     int buf = 0;
     for (int t = tl; t >= t0; t -= SEG, buf ^= 1) {
         Ci.store(sC[buf], tid);
@@ -156,11 +154,9 @@ template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds_
     const int left_ch = p.dg - (cb - ch.g * p.cbg) * CH, d0 = ch.g * p.dg + p.dg - left_ch;
     float A2[K], dAs[K], dsks = 0.0f, dbss = 0.0f;      // sums over blocks of 256 steps; a block's own come first, so that long sums stay exact
     load_states<K>(p.A + (int64_t)d * p.N, ch.n, p.N, p.vec, A2);
+    decay_rates<K>(A2);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        A2[k] *= SNN_LOG2E;
-        dAs[k] = 0.0f;
-    }
+    for (int k = 0; k < K; ++k) dAs[k] = 0.0f;
     const float bias = p.dbias ? p.dbias[d] : 0.0f, skip = p.skip ? p.skip[d] : 0.0f;
     const int64_t rows = p.seq.offsets ? p.seq.n_rows : (int64_t)p.seq.n_seq * p.seq.max_T;
     float* bcpart = p.bcpart ? p.bcpart + (int64_t)cb * rows * (2 * NP) : nullptr;

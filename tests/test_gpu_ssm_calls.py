@@ -77,3 +77,41 @@ def test_small_states_that_grow_over_a_chunk():
     R.close(_np(gr.dA), ref["dA"], mag["dA"], 2 * k + T, what="dA")
     for name, got in (("dB", gr.dB[0]), ("dC", gr.dC[0])):
         R.close(_np(got), ref[name].sum(1), mag[name].sum(1), 2 * k + D, what=name)
+
+
+@pytest.mark.parametrize("low", [-float("inf"), -3.4e38])
+@pytest.mark.parametrize("T", [5, 301])
+def test_decays_of_the_lowest_value(low, T):
+    """exp(s A) is 0 for every step s > 0 and 1 for a step of zero of a finite A, and the steps that fill up the last segment leave
+    the state as it is.  In 64 bits -1e30 says the same."""
+    g = torch.Generator().manual_seed(T)
+    D, N = 6, 4
+    rnd = lambda *s: torch.randn(s, generator=g).cuda()                                           # noqa: E731
+    x, delta, B, C, dy = rnd(1, T, D), rnd(1, T, D), rnd(1, T, N), rnd(1, T, N), rnd(1, T, D)
+    A = -torch.rand(D, N, generator=g).cuda() - 0.1
+    finite = A.clone()
+    finite[1], finite[:, 2] = -1e30, -1e30
+    A[1], A[:, 2] = low, low
+    if low > -float("inf"):
+        delta[:, 3] = -200.0                         # softplus: 0
+    kw = dict(time_major=False)
+    y, end, tape = ssm.selective_scan_train(x, delta, A, B, C, want_final_state=True, **kw)
+    wide = lambda t: np.repeat(_np(t[0])[:, None], D, axis=1)                                     # noqa: E731
+    args, rkw = (_np(x[0]), _np(delta[0]), _np(finite), wide(B), wide(C)), dict(dy=_np(dy[0]))
+    # softplus(-200) = 1e-87 in 64 bits, and 1e-87 x 1e30 is still nothing
+    ref, mag = R.scan(*args, **rkw), R.scan(*args, mag=True, **rkw)
+    k = 16 * T + 32
+    R.close(_np(y[0]), ref["y"], mag["y"], k, what="y")
+    R.close(_np(end[0]), ref["end"], mag["end"], k, what="end")
+    if low > -float("inf"):                          # the slope of exp(s A) at -inf is 0 x inf
+        gr = ssm.selective_scan_backward(x, delta, A, B, C, dy, tape, **kw)
+        for name, got in (("dx", gr.dx[0]), ("ddelta", gr.ddelta[0])):
+            R.close(_np(got), ref[name], mag[name], 2 * k, what=name)
+        R.close(_np(gr.dA), ref["dA"], mag["dA"], 2 * k + T, what="dA")
+    state, want = rnd(1, D, N), None
+    s0 = state.clone()
+    y1 = ssm.selective_scan_step(x[:, 3], state, delta[:, 3], A, B[:, 3], C[:, 3])
+    one = R.scan(*(a[3:4] if i != 2 else a for i, a in enumerate(args)), h0=_np(s0[0]))
+    m1 = R.scan(*(a[3:4] if i != 2 else a for i, a in enumerate(args)), h0=_np(s0[0]), mag=True)
+    R.close(_np(y1), one["y"], m1["y"], 48, what="step y")
+    R.close(_np(state[0]), one["end"], m1["end"], 48, what="step end")
