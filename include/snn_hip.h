@@ -488,7 +488,7 @@ int snn_sgd_step_clipped(int64_t n, float *params, const float *grads, float *mo
  * kernels only; values out of range are cut to the tensors (a length to [0, max_T], an offset to [0, n_rows]).
  * Rows that belong to no step -- behind a sequence's end in a padded batch, outside every sequence among ragged rows, past
  * max_T -- are never read, and zero in every output.  A sequence of length 0 hands its initial state on.  Offsets must not
- * decrease (rows that two sequences share have no defined result).  At most 2^24 - 1 sequences, 2^30 steps, 2^19 channels.
+ * decrease (the results of a batch whose offsets do are not defined; nothing outside the tensors is touched).  At most 2^24 - 1 sequences, 2^30 steps, 2^19 channels.
  */
 typedef struct snn_seq {
     int32_t n_seq, max_T;

@@ -27,8 +27,15 @@ template <typename T> struct ConvP {
     T *s_out, *ds_in;
     float* part;
     int D, cv, tc, nc, slots, silu;     // channels, vectors per row, steps per chunk, chunks per sequence, backward: item slots
+    int sh;                             // < 0: items are (sequence, chunk) of a grid of nc a sequence; else of seq_find_item, tc = 2^sh
     int64_t items;
 };
+template <typename T> __device__ __forceinline__ SeqItem chunk_of(const ConvP<T>& p, int64_t item)
+{
+    if (p.sh >= 0) return seq_find_item(p.seq, item, p.sh);
+    const int b = (int)(item / p.nc);
+    return SeqItem{b, item - (int64_t)b * p.nc};
+}
 
 template <typename T, int V> __device__ __forceinline__ void load_v(const T* p, float (&v)[V])
 {
@@ -80,9 +87,12 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= p.items * p.cv) return;
     const int64_t item = id / p.cv;
-    const int d = (int)(id - item * p.cv) * V, b = (int)(item / p.nc), c = (int)(item - (int64_t)b * p.nc);
+    const SeqItem it = chunk_of(p, item);
+    const int64_t c = it.c;
+    if (c < 0) return;
+    const int d = (int)(id - item * p.cv) * V, b = it.b;
     const SeqRange r = seq_range(p.seq, b);
-    const int t0 = c * p.tc, t1 = t0 + p.tc < r.len ? t0 + p.tc : r.len;
+    const int t0 = c * p.tc < r.len ? (int)(c * p.tc) : r.len, t1 = t0 + p.tc < r.len ? t0 + p.tc : r.len;
     const int64_t xb = r.row0 * p.x.st + b * p.x.sb + d, yb = r.row0 * p.y.st + b * p.y.sb + d;
     if (t0 < t1) {
         float wt[W][V], bs[V], win[W][V];
@@ -125,7 +135,7 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
             store_v<T, V>(p.s_out + ((int64_t)b * (W - 1) + k) * p.D + d, v);
         }
     }
-    clear_rows<T, V>(p.y, fill_range(p.seq, r, b, t0, t0 + p.tc, c == p.nc - 1), yb);
+    clear_rows<T, V>(p.y, fill_of_chunk(p.seq, r, b, c, p.tc, p.sh < 0 && c == p.nc - 1), yb);
 }
 
 // A thread takes the chunks slot, slot + slots, .. so that the parameter gradients of many sequences add up in registers;
@@ -141,9 +151,12 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
 #pragma unroll
     for (int k = 0; k < W; ++k) zero_v(dws[k]);
     for (int64_t item = slot; item < p.items; item += p.slots) {
-        const int b = (int)(item / p.nc), c = (int)(item - (int64_t)b * p.nc);
+        const SeqItem it = chunk_of(p, item);
+        const int b = it.b;
+        const int64_t c = it.c;
+        if (c < 0) continue;
         const SeqRange r = seq_range(p.seq, b);
-        const int t0 = c * p.tc, t1 = t0 + p.tc < r.len ? t0 + p.tc : r.len;
+        const int t0 = c * p.tc < r.len ? (int)(c * p.tc) : r.len, t1 = t0 + p.tc < r.len ? t0 + p.tc : r.len;
         const int64_t xb = r.row0 * p.x.st + b * p.x.sb + d, gb = r.row0 * p.dy.st + b * p.dy.sb + d;
         const int64_t ob = r.row0 * p.dx.st + b * p.dx.sb + d;
         if (t0 < t1 || c == 0) {                    // c == 0: the gradient of the initial state, also of an empty sequence
@@ -236,7 +249,7 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
                 dbs[i] += db[i];
             }
         }
-        clear_rows<T, V>(p.dx, fill_range(p.seq, r, b, t0, t0 + p.tc, c == p.nc - 1), ob);
+        clear_rows<T, V>(p.dx, fill_of_chunk(p.seq, r, b, c, p.tc, p.sh < 0 && c == p.nc - 1), ob);
     }
     float* q = p.part + (int64_t)slot * (W + 1) * p.D + d;
 #pragma unroll
@@ -321,24 +334,31 @@ int vector_width(const snn_conv_args* a, int what)
     if (what != BWD) ptr(a->state_out);
     return ok ? v : 1;
 }
+// Items of chunks of t steps.  A grid of max_T's chunks for every sequence, or, where more than half of that of ragged rows would be
+// empty (one long sequence among short ones, or no bound known but the number of rows), the chunks that the rows can have, each of
+// which then searches its sequence.  Grid / search, forward and backward: 4000 x up to 40 x 64 fp32 (grid 1.3 times the search's items)
+// 11 / 18 and 39 / 50 us, 256 x up to 300 x 256 fp32 (1.8) 17.7 / 18.7 and 43 / 41, 7 x up to 1501 x 1536 fp16 (1.9) 15.8 / 12.2 and
+// 36 / 27, 8192 + 7 x 64 x 4096 bf16 (7) 42 / 38 and 133 / 71.
+int64_t grid_items(const snn_seq& s, int t) { return (int64_t)s.n_seq * ((s.max_T + t - 1) / t); }
+int64_t row_items(const snn_seq& s, int t) { return s.n_rows / t + s.n_seq; }
+bool by_rows(const snn_seq& s, int t) { return s.offsets && grid_items(s, t) > 2 * row_items(s, t); }
+int64_t item_count(const snn_seq& s, int t) { return by_rows(s, t) ? row_items(s, t) : grid_items(s, t); }
+
 // Steps per chunk: the longest of 64 (backward: 128) .. 16 that leaves 2^17 threads (two waves on every SIMD), so that long
 // chunks (few repeated rows) go to large batches and short ones to single sequences.  Forward of 2048 x 300 x 256 fp32 with up
 // to 64 / 128 / 512 steps: 193 / 208 / 206 us.
-void chunks(const snn_conv_args* a, int v, int what, int* tc, int* nc)
+int chunk_steps(const snn_conv_args* a, int v, int what)
 {
     const int64_t cv = (a->channels + v - 1) / v;
     int t = what == BWD ? 128 : 64;
-    while (t > 16 && (int64_t)a->seq.n_seq * ((a->seq.max_T + t - 1) / t) * cv < (1 << 17)) t >>= 1;
-    *tc = t;
-    *nc = (a->seq.max_T + t - 1) / t;
+    while (t > 16 && item_count(a->seq, t) * cv < (1 << 17)) t >>= 1;
+    return t;
 }
 // Backward slots: about 2^17 threads (what its registers let the chip hold), never more than there are chunks.  2^18 take the
 // same time and leave twice the partial sums: 18 instead of 10 us of adding up.
 int bwd_slots(const snn_conv_args* a, int v)
 {
-    int tc, nc;
-    chunks(a, v, BWD, &tc, &nc);
-    const int64_t cv = (a->channels + v - 1) / v, items = (int64_t)a->seq.n_seq * nc;
+    const int64_t cv = (a->channels + v - 1) / v, items = item_count(a->seq, chunk_steps(a, v, BWD));
     return (int)std::max<int64_t>(1, std::min<int64_t>(items, ((1 << 17) + cv - 1) / cv));
 }
 
@@ -361,9 +381,10 @@ template <typename T, int V, int W> int launch(const snn_conv_args* a, int what,
     p.cv = (a->channels + V - 1) / V;
     p.silu = a->silu;
     p.slots = 0;
-    chunks(a, V, what, &p.tc, &p.nc);
-    if (what == STEP) p.tc = p.nc = 1;
-    p.items = (int64_t)a->seq.n_seq * p.nc;
+    p.tc = what == STEP ? 1 : chunk_steps(a, V, what);
+    p.sh = by_rows(a->seq, p.tc) ? __builtin_ctz(p.tc) : -1;
+    p.nc = (a->seq.max_T + p.tc - 1) / p.tc;
+    p.items = item_count(a->seq, p.tc);
     if (what == BWD) p.slots = bwd_slots(a, V);
     const int64_t blocks = ((what == BWD ? (int64_t)p.slots : p.items) * p.cv + 255) / 256;
     if (blocks > SEQ_MAX_BLOCKS) { snn_set_error("convolution: %lld workgroups", (long long)blocks); return SNN_ERR_UNSUPPORTED; }

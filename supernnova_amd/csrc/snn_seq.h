@@ -55,6 +55,37 @@ __device__ __forceinline__ SeqRange seq_range(const snn_seq& s, int b)
     }
     return r;
 }
+// Chunks of 2^sh steps as work items of a ragged batch: sequence b has the items from (offsets[b] >> sh) + b on, room for its every
+// step, so that (n_rows >> sh) + n_seq hold all of them whatever bound on the lengths the caller knows; the last sequence has the
+// rest, enough for the rows behind it.
+struct SeqItem { int b; int64_t c; };                  // sequence, chunk
+__device__ __forceinline__ int64_t seq_first_item(const snn_seq& s, int b, int sh)
+{
+    const int64_t o = s.offsets[b];
+    return ((o < 0 ? 0 : (o > s.n_rows ? s.n_rows : o)) >> sh) + b;
+}
+// Which sequence an item of ragged rows belongs to: the last one whose first item is not behind it, by a search that asks seven
+// places at once (a search by halves waits for log2 n_seq loads one after the other).  Offsets that decrease find some sequence, and
+// maybe a chunk below 0, which the caller leaves out.
+__device__ __forceinline__ SeqItem seq_find_item(const snn_seq& s, int64_t item, int sh)
+{
+    int lo = 0, hi = s.n_seq;                          // in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 7) >> 3;
+        int n = 0;
+#pragma unroll
+        for (int k = 1; k < 8; ++k) {
+            const int b = lo + k * step;
+            n += b < hi && seq_first_item(s, b < hi ? b : lo, sh) <= item;
+        }
+        hi = lo + (n + 1) * step < hi ? lo + (n + 1) * step : hi;
+        lo += n * step;
+    }
+    SeqItem r;
+    r.b = lo;
+    r.c = item - seq_first_item(s, lo, sh);
+    return r;
+}
 // Rows (relative to row0) that belong to no step and that chunk [t0, t1) of sequence b has to clear, as two ranges:
 // behind the sequence's end inside the padded batch, and -- ragged rows -- before the first and behind the last sequence.
 struct FillRange { int64_t a0, a1, b0, b1; };
@@ -71,6 +102,15 @@ __device__ __forceinline__ FillRange fill_range(const snn_seq& s, const SeqRange
         f.a0 = r.len > t0 ? r.len : t0;
         f.a1 = last_chunk ? s.max_T : t1;
     }
+    return f;
+}
+
+// The same where every chunk c of tc steps clears its own steps' worth, and the sequence's last one (`last`, if any is) all behind.
+__device__ __forceinline__ FillRange fill_of_chunk(const snn_seq& s, const SeqRange& r, int b, int64_t c, int tc, bool last)
+{
+    const int64_t t0 = c * tc, end = s.offsets ? (b == s.n_seq - 1 ? s.n_rows : r.end) - r.row0 : s.max_T;
+    FillRange f = {r.len > t0 ? r.len : t0, last || end < t0 + tc ? end : t0 + tc, 0, 0};
+    if (s.offsets && b == 0 && c == 0) f.b0 = -r.row0;
     return f;
 }
 

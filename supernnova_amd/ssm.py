@@ -10,10 +10,11 @@ may be strided (a slice of a wider projection needs no copy):
     (T, B, D)  time_major=True (default), padded, `lengths` int32 (B,) on the device or None
     (B, T, D)  time_major=False, padded, `lengths` likewise
     (R, D)     ragged rows, `offsets` int64 (B + 1,) on the device: sequence b holds rows offsets[b] .. offsets[b + 1];
-               `max_len`: a bound on the lengths known to the host (default: the number of rows; a good one saves workspace)
+               `max_len`: a bound on the lengths known to the host (default: the number of rows; the scan splits the time axis by it,
+               so a loose one costs time)
 Rows that belong to no step (behind a sequence's end, outside every sequence, past max_len) are never read, and zero in every
 output.  A sequence of length 0 hands its initial state on.  Lengths and offsets stay on the device (no synchronisation);
-values out of range are cut to the tensors.  Offsets must not decrease: rows that two sequences share have no defined result.
+values out of range are cut to the tensors.  Offsets must not decrease: the results of a batch whose offsets do are not defined.
 
 x, delta, z, B, C and what has their shape are float32, bfloat16 or float16, one type per call; parameters, their gradients and
 scan states are float32, sums and states are held in float32, and results are rounded once.  B and C are (.., N) or, with

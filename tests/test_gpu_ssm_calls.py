@@ -115,3 +115,64 @@ def test_decays_of_the_lowest_value(low, T):
     m1 = R.scan(*(a[3:4] if i != 2 else a for i, a in enumerate(args)), h0=_np(s0[0]), mag=True)
     R.close(_np(y1), one["y"], m1["y"], 48, what="step y")
     R.close(_np(state[0]), one["end"], m1["end"], 48, what="step end")
+
+
+def _many(B, D, dt, g):
+    lens = torch.randint(0, 4, (B,), generator=g)
+    lens[B // 2] = 300
+    off = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)]).cuda()
+    return lens, off, torch.randn(int(off[-1]) + 7, D, generator=g).to(dt).cuda()
+
+
+@pytest.mark.parametrize("B,D,dt", [(1 << 20, 1, torch.float32), (5000, 64, torch.bfloat16), (300, 20, torch.float16)])
+def test_conv_of_many_sequences_without_max_len(B, D, dt):
+    """The bound that max_len defaults to, the number of rows, is as good as the true one: the same bits."""
+    g = torch.Generator().manual_seed(B)
+    lens, off, x = _many(B, D, dt, g)
+    x[off[-1]:] = float("nan")
+    dy = torch.randn(x.shape, generator=g).to(dt).cuda()
+    w, bias = torch.randn(D, 4, generator=g).cuda(), torch.randn(D, generator=g).cuda()
+    s0, ds = torch.randn(B, 3, D, generator=g).to(dt).cuda(), torch.randn(B, 3, D, generator=g).to(dt).cuda()
+    outs = []
+    for max_len in (None, 300):
+        y, end = ssm.causal_conv_forward(x, w, bias, offsets=off, max_len=max_len, initial_state=s0, want_final_state=True)
+        gr = ssm.causal_conv_backward(x, w, bias, dy, dfinal_state=ds, offsets=off, max_len=max_len, initial_state=s0)
+        outs.append([y, end, *gr])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert (outs[0][0][off[-1]:] == 0).all() and (outs[0][2][off[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize("dt,D,W", [("f32", 24, 4), ("bf16", 64, 3), ("f16", 7, 2)])
+@pytest.mark.parametrize("max_len", [None, 150])
+def test_conv_of_rows_that_are_mostly_one_sequence(dt, D, W, max_len):
+    """One long sequence among short and empty ones, rows before the first and behind the last, and rows past max_len: values and
+    gradients of every sequence, zeros in every row that belongs to no step."""
+    g = torch.Generator().manual_seed(D)
+    T = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dt]
+    lens, front, back = [0, 2, 200, 1, 0, 3, 0], 5, 40
+    off = np.cumsum([front] + lens)
+    R_ = int(off[-1]) + back
+    x, dy = (torch.randn(R_, D, generator=g).to(T) for _ in range(2))
+    dead = np.ones(R_, bool)
+    for b, n in enumerate(lens):
+        dead[off[b]:off[b] + min(n, max_len or n)] = False
+    x[dead], dy[dead] = float("nan"), float("nan")
+    x, dy, w, bias = x.cuda(), dy.cuda(), torch.randn(D, W, generator=g).cuda(), torch.randn(D, generator=g).cuda()
+    s0, ds = (torch.randn(len(lens), W - 1, D, generator=g).to(T).cuda() for _ in range(2))
+    kw = dict(offsets=torch.tensor(off).cuda(), max_len=max_len, initial_state=s0)
+    y, end = ssm.causal_conv_forward(x, w, bias, want_final_state=True, **kw)
+    gr = ssm.causal_conv_backward(x, w, bias, dy, dfinal_state=ds, **kw)
+    assert (_np(y)[dead] == 0).all() and (_np(gr.dx)[dead] == 0).all()
+    k, parts, mags = W + 16, [], []
+    for b, n in enumerate(lens):
+        at = slice(off[b], off[b] + min(n, max_len or n))
+        a = (_np(x)[at], _np(w), _np(bias), True, _np(s0[b]), _np(dy)[at], _np(ds[b]))
+        r, m = R.conv(*a), R.conv(*a, mag=True)
+        R.close(_np(y)[at], r["y"], m["y"], k, dt, "y")
+        R.close(_np(end[b]), r["end"], m["end"], 0, dt, "end")
+        R.close(_np(gr.dx)[at], r["dx"], m["dx"], 2 * k, dt, "dx")
+        R.close(_np(gr.dinitial_state[b]), r["ds0"], m["ds0"], 2 * k, dt, "ds0")
+        parts.append(r)
+        mags.append(m)
+    for name, got in (("dw", gr.dweight), ("db", gr.dbias)):       # a chunk's at most 16 steps in fp32, chunks of a slot, then fp64
+        R.close(_np(got), sum(p[name] for p in parts), sum(p[name] for p in mags), 2 * k + 16 + 32, "f32", name)
