@@ -196,7 +196,8 @@ def train_swag(settings, list_data_train=None, list_data_val=None):
 
 def train_swag_finetune(settings, list_data_train=None, list_data_val=None):
     """SWAG fine-tuning (train_rnn.py:516-663): load `settings.swag_pretrained_path` into a fresh model, train it with
-    SGD (momentum 0.9, weight decay 1e-4 -- hard-coded in the reference, :541-546) for 30 epochs (:548-549), enter every
+    SGD (momentum 0.9, weight decay 1e-4 -- hard-coded in the reference, :541-546; settings.max_grad_norm as in
+    get_optimizer) for 30 epochs (:548-549), enter every
     epoch's parameters into the SwagModel statistics and evaluate / save SWAG draws from the third epoch on.
     The reference unpickles the pre-trained file (torch.load(..., weights_only=False), :537); here it must be a plain
     state dict, read with weights_only=True.  Returns (rnn, swag_rnn)."""
@@ -213,7 +214,8 @@ def train_swag_finetune(settings, list_data_train=None, list_data_val=None):
     if settings.use_cuda:
         rnn.cuda()
         swag_rnn.cuda()
-    optimizer = FusedSGD(rnn, lr=settings.learning_rate, momentum=0.9, weight_decay=1e-4)
+    optimizer = FusedSGD(rnn, lr=settings.learning_rate, momentum=0.9, weight_decay=1e-4,
+                         max_grad_norm=getattr(settings, "max_grad_norm", None))
     d_train, d_val = _monitors(settings)
     best_loss, t_start = float("inf"), time()
     for epoch in range(settings.nb_epoch):
