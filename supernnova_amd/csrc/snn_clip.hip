@@ -18,6 +18,7 @@
 #include <new>
 #include "snn_host.h"
 #include "snn_seq.h"
+#include "snn_update.h"
 
 #define HIP_CHECK(x) do { hipError_t e_ = (x); if (e_ != hipSuccess) { \
     snn_set_error("%s: %s", #x, hipGetErrorString(e_)); return SNN_ERR_HIP; } } while (0)
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(const Table t, const do
     else scale_piece<f16_t>((const f16_t*)t.src[ti] + at, (f16_t*)t.dst[ti] + at, n, c);
 }
 
-// The updates of snn_adam_step and snn_sgd_step (snn_train.hip), gradients multiplied by grad_scale * *coef: the coefficient is
+// The updates of snn_adam_step and snn_sgd_step (snn_update.h), gradients multiplied by grad_scale * *coef: the coefficient is
 // read where clip_finish_kernel left it, so a clipped step reads the gradient twice and never writes it.
 __global__ void __launch_bounds__(256) adam_clipped_kernel(int64_t n, float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
                                                           float* __restrict__ v, float lr, float beta1, float beta2, float eps, float weight_decay,
@@ -186,13 +187,7 @@ __global__ void __launch_bounds__(256) adam_clipped_kernel(int64_t n, float* __r
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
-    const float pi = p[i];
-    float gi = g[i] * grad_scale * *coef;
-    if (weight_decay != 0.0f) gi = fmaf(weight_decay, pi, gi);
-    const float mi = m[i] + (gi - m[i]) * (1.0f - beta1), vi = beta2 * v[i] + (1.0f - beta2) * gi * gi;
-    m[i] = mi;
-    v[i] = vi;
-    p[i] = pi - (lr / bc1) * (mi / (sqrtf(vi) / bc2_sqrt + eps));
+    adam_update(g[i] * grad_scale * *coef, p, m, v, i, lr, beta1, beta2, eps, weight_decay, bc1, bc2_sqrt);
 }
 __global__ void __launch_bounds__(256) sgd_clipped_kernel(int64_t n, float* __restrict__ p, const float* __restrict__ g, float* __restrict__ buf,
                                                          float lr, float momentum, float weight_decay, int first, float grad_scale,
@@ -200,14 +195,7 @@ __global__ void __launch_bounds__(256) sgd_clipped_kernel(int64_t n, float* __re
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
-    const float pi = p[i];
-    float gi = g[i] * grad_scale * *coef;
-    if (weight_decay != 0.0f) gi = fmaf(weight_decay, pi, gi);
-    if (momentum != 0.0f) {
-        gi = first ? gi : fmaf(momentum, buf[i], gi);
-        buf[i] = gi;
-    }
-    p[i] = pi - lr * gi;
+    sgd_update(g[i] * grad_scale * *coef, p, buf, i, lr, momentum, weight_decay, first);
 }
 
 int64_t pieces_of(int64_t n) { return (n + CLIP_PIECE - 1) / CLIP_PIECE; }

@@ -13,6 +13,7 @@
 
 #include "snn_kernels.h"
 #include "snn_host.h"
+#include "snn_update.h"
 
 #define HIP_CHECK(expr)                                                             \
     do {                                                                            \
@@ -357,15 +358,7 @@ __global__ void __launch_bounds__(256) adam_kernel(int64_t n, float* __restrict_
 {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
-    float gi = g[i] * grad_scale;
-    const float pi = p[i];
-    if (weight_decay != 0.0f) gi = fmaf(weight_decay, pi, gi);
-    const float mi = m[i] + (gi - m[i]) * (1.0f - beta1);          // lerp, as torch
-    const float vi = beta2 * v[i] + (1.0f - beta2) * gi * gi;
-    m[i] = mi;
-    v[i] = vi;
-    const float denom = sqrtf(vi) / bc2_sqrt + eps;
-    p[i] = pi - (lr / bc1) * (mi / denom);
+    adam_update(g[i] * grad_scale, p, m, v, i, lr, beta1, beta2, eps, weight_decay, bc1, bc2_sqrt);
 }
 
 extern "C" int snn_adam_step(int64_t n, float* params, const float* grads, float* exp_avg, float* exp_avg_sq,
@@ -394,14 +387,7 @@ __global__ void __launch_bounds__(256) sgd_kernel(int64_t n, float* __restrict__
 {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
-    const float pi = p[i];
-    float gi = g[i] * grad_scale;
-    if (weight_decay != 0.0f) gi = fmaf(weight_decay, pi, gi);
-    if (momentum != 0.0f) {
-        gi = first ? gi : fmaf(momentum, buf[i], gi);      // the first step copies the gradient into the buffer
-        buf[i] = gi;
-    }
-    p[i] = pi - lr * gi;
+    sgd_update(g[i] * grad_scale, p, buf, i, lr, momentum, weight_decay, first);
 }
 
 extern "C" int snn_sgd_step(int64_t n, float* params, const float* grads, float* momentum_buf, int64_t step, float lr,
