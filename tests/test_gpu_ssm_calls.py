@@ -7,6 +7,7 @@ import torch
 import ssm_reference as R
 from supernnova_amd import engine as E
 from supernnova_amd import ssm
+from test_gpu_ssm import Batch, _check_scan, _scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -176,3 +177,153 @@ def test_conv_of_rows_that_are_mostly_one_sequence(dt, D, W, max_len):
         mags.append(m)
     for name, got in (("dw", gr.dweight), ("db", gr.dbias)):       # a chunk's at most 16 steps in fp32, chunks of a slot, then fp64
         R.close(_np(got), sum(p[name] for p in parts), sum(p[name] for p in mags), 2 * k + 16 + 32, "f32", name)
+
+
+def _scan64(i, h0, dy, dend, live, mag=False):
+    """ssm_reference.scan over a whole (T, B, D) batch in torch float64, one group, softplus; `live` (T, B, 1)."""
+    f = torch.abs if mag else (lambda v: v)
+    x, z, B, C, dy = (torch.where(live, i[k].double() if k else dy.double(), 0.0) for k in ("x", "z", "B", "C", None))
+    v = i["delta"].double() + i["delta_bias"].double()
+    s, sig = torch.where(live, torch.nn.functional.softplus(v), 0.0), torch.sigmoid(v)
+    A, skip = i["A"].double(), f(i["D"].double())
+    T = x.shape[0]
+    e = torch.sigmoid(z)
+    gate = f(z * e)
+    hs, ys, a = [f(h0.double())], [], [torch.exp(s[t, :, :, None] * A) for t in range(T)]
+    for t in range(T):
+        hs.append(a[t] * hs[-1] + (s[t] * f(x[t]))[..., None] * f(B[t])[:, None])
+        ys.append((hs[-1] * f(C[t])[:, None]).sum(-1) + skip * f(x[t]))
+    y = torch.stack(ys)
+    g = f(dy) * gate
+    out = dict(y=y * gate, end=hs[T], dz=f(dy) * y * (f(e * (1 + z * (1 - e))) + (1.0 if mag else 0.0)))
+    w, r = f(dend.double()), {k: [] for k in ("dx", "ddelta", "dB", "dC")}
+    dA = torch.zeros_like(A)
+    for t in range(T - 1, -1, -1):
+        q = torch.where(live[t][..., None], f(C[t])[:, None] * g[t][..., None], 0.0) + w
+        qb, w = (q * f(B[t])[:, None]).sum(-1), a[t] * q
+        wh = w * hs[t]
+        dA += (wh * s[t][..., None]).sum(0)
+        r["ddelta"].append(torch.where(live[t], (f(x[t]) * qb + (wh * f(A)).sum(-1)) * sig[t], 0.0))
+        r["dx"].append(skip * g[t] + s[t] * qb)
+        r["dB"].append((q * (s[t] * f(x[t]))[..., None]).sum(1))
+        r["dC"].append((hs[t + 1] * g[t][..., None]).sum(1))
+    out.update({k: torch.stack(u[::-1]) for k, u in r.items()}, dA=dA, dinitial_state=w, dD=(g * f(x)).sum((0, 1)))
+    out["ddelta_bias"] = out["ddelta"].sum((0, 1))
+    return out
+
+
+@pytest.mark.parametrize("B,D,N,layout", [(3000, 64, 16, "time"), (5000, 70, 16, "batch"), (4500, 40, 5, "rows"), (2600, 20, 40, "time")])
+def test_scan_gradients_of_more_chunks_than_workgroups(B, D, N, layout):
+    """A workgroup takes several sequences (with up to 4096 of them longest first) and adds their parameter gradients up.  All
+    inputs are positive, so that one sequence too few or too many is 1 / B of a sum, four times the tolerance."""
+    T = 6
+    g = torch.Generator().manual_seed(B)
+    rnd = lambda *s: torch.randn(s, generator=g).abs().cuda()                                     # noqa: E731
+    lens = torch.randint(0, T + 1, (B,), generator=g).cuda()
+    i = dict(x=rnd(T, B, D), delta=rnd(T, B, D) * 0.7, A=-rnd(D, N) - 0.1, B=rnd(T, B, N), C=rnd(T, B, N), D=rnd(D), z=rnd(T, B, D), delta_bias=rnd(D) * 0.5)
+    dy, h0, dend = rnd(T, B, D), rnd(B, D, N), rnd(B, D, N)
+    live = (torch.arange(T, device="cuda")[:, None] < lens)[..., None]
+    per = ("x", "delta", "B", "C", "z")
+    if layout == "rows":
+        lay = lambda t: t.transpose(0, 1)[live[..., 0].t()].contiguous()                          # noqa: E731
+        kw = dict(offsets=torch.cat([lens.new_zeros(1), lens.cumsum(0)]), max_len=T)
+    else:
+        lay = (lambda t: t) if layout == "time" else (lambda t: t.transpose(0, 1).contiguous())
+        kw = dict(lengths=lens.int(), time_major=layout == "time")
+    j, kw = {k: lay(v) if k in per else v for k, v in i.items()}, dict(kw, initial_state=h0)
+    y, end, tape = ssm.selective_scan_train(**j, want_final_state=True, **kw)
+    gr = ssm.selective_scan_backward(**j, dy=lay(dy), tape=tape, dfinal_state=dend, **kw)
+    ref, mag = _scan64(i, h0, dy, dend, live), _scan64(i, h0, dy, dend, live, mag=True)
+    k = 16 * T + 32 + N
+    joins = -(-B // (2048 // -(-D // (256 // (4 if N <= 16 else 16)))))           # sequences a workgroup adds up in fp32
+    tight = 2 * k + T + joins
+    assert 4 * tight * R.EPS32 < 1 / B
+    for name, got in [("y", y), ("end", end), *zip(gr._fields, gr)]:
+        rows = name in ("y", "dx", "ddelta", "dz", "dB", "dC")
+        r, m = (lay(torch.where(live, v[name], 0.0)) if rows else v[name] for v in (ref, mag))
+        n = {"y": k, "end": k, "dA": tight, "dD": tight, "ddelta_bias": tight, "dB": 2 * k + D, "dC": 2 * k + D}.get(name, 2 * k)
+        R.close(_np(got), _np(r), _np(m), n, "f32", name)
+
+
+@pytest.mark.parametrize("B,T,D,dt,layout", [(1200, 300, 128, "f32", "time"), (70000, 10, 32, "f32", "batch"), (9000, 40, 64, "bf16", "rows")])
+def test_conv_gradients_of_more_chunks_than_slots(B, T, D, dt, layout):
+    """Chunks of more than 16 steps, several of which a thread adds up.  All inputs are positive: one chunk too few or too many is
+    more than the tolerance."""
+    W, g = 4, torch.Generator().manual_seed(B)
+    dtype = {"f32": torch.float32, "bf16": torch.bfloat16}[dt]
+    rnd = lambda *s: torch.randn(s, generator=g).abs().cuda()                                     # noqa: E731
+    lens = torch.randint(0, T + 1, (B,), generator=g).cuda()
+    x, dy, s0, ds = (rnd(*s).to(dtype) for s in ((T, B, D), (T, B, D), (B, W - 1, D), (B, W - 1, D)))
+    w, bias = rnd(D, W) / 2, rnd(D)
+    live = (torch.arange(T, device="cuda")[:, None] < lens)[..., None]
+    if layout == "rows":
+        lay = lambda t: t.transpose(0, 1)[live[..., 0].t()].contiguous()                          # noqa: E731
+        kw = dict(offsets=torch.cat([lens.new_zeros(1), lens.cumsum(0)]), max_len=T)
+    else:
+        lay = (lambda t: t) if layout == "time" else (lambda t: t.transpose(0, 1).contiguous())
+        kw = dict(lengths=lens.int(), time_major=layout == "time")
+    gr = ssm.causal_conv_backward(lay(x), w, bias, lay(dy), dfinal_state=ds, initial_state=s0, **kw)
+    xx = torch.cat([s0.double().transpose(0, 1), torch.where(live, x.double(), 0.0)])
+    p = bias.double() + sum(w[:, k].double() * xx[k:k + T] for k in range(W))
+    sg = torch.sigmoid(p)
+    dp = torch.where(live, dy.double() * sg * (1 + p * (1 - sg)), 0.0)
+    mag = torch.where(live, dy.double() * (sg * (1 + p * (1 - sg)).abs() + p), 0.0)
+    dw = [torch.stack([(v * xx[k:k + T]).sum((0, 1)) for k in range(W)], 1) for v in (dp, mag)]
+    dxx = [torch.zeros_like(xx), torch.zeros_like(xx)]
+    for d, v in zip(dxx, (dp, mag)):
+        for k in range(W):
+            d[k:k + T] += w[:, k].double() * v
+        d.scatter_add_(0, (lens[None] + torch.arange(W - 1, device="cuda")[:, None])[..., None].expand(W - 1, B, D), ds.double().transpose(0, 1))
+    k = W + 16
+    tight = 2 * k + 128 + 8                          # a chunk's steps and the joins of a thread in fp32, then fp64
+    R.close(_np(gr.dweight), _np(dw[0]), _np(dw[1]), tight, "f32", "dweight")
+    R.close(_np(gr.dbias), _np(dp.sum((0, 1))), _np(mag.sum((0, 1))), tight, "f32", "dbias")
+    R.close(_np(gr.dinitial_state), *(_np(d[:W - 1].transpose(0, 1)) for d in dxx), 2 * k, dt, "dinitial_state")
+    R.close(_np(gr.dx), *(_np(lay(torch.where(live, d[W - 1:], 0.0))) for d in dxx), 2 * k, dt, "dx")
+
+
+def test_scan_split_over_time_agrees_with_the_whole():
+    """Two sequences of 700 steps, whose time axis is split, and the same among 256, which fill the chip and are not."""
+    T, D, N, many = 700, 96, 16, 128
+    g = torch.Generator().manual_seed(11)
+    rnd = lambda *s: torch.randn(s, generator=g)                                                  # noqa: E731
+    i = dict(x=rnd(2, T, D), delta=rnd(2, T, D) * 0.7, B=rnd(2, T, N), C=rnd(2, T, N), z=rnd(2, T, D), A=-torch.rand(D, N, generator=g) * 2 - 0.1,
+             D=rnd(D), delta_bias=rnd(D) * 0.5)
+    dy, h0, dend, lens = rnd(2, T, D), rnd(2, D, N), rnd(2, D, N), torch.tensor([700, 650], dtype=torch.int32)
+    runs = []
+    for n in (1, many):
+        rep = lambda t: t.repeat(n, *[1] * (t.dim() - 1)).cuda()                                  # noqa: E731
+        j = {k: rep(v) if k not in ("A", "D", "delta_bias") else v.cuda() for k, v in i.items()}
+        kw = dict(initial_state=rep(h0), lengths=rep(lens), time_major=False)
+        y, end, tape = ssm.selective_scan_train(**j, want_final_state=True, **kw)
+        gr = ssm.selective_scan_backward(**j, dy=rep(dy), tape=tape, dfinal_state=rep(dend), **kw)
+        runs.append(dict(y=y[:2], end=end[:2], dx=gr.dx[:2], ddelta=gr.ddelta[:2], dz=gr.dz[:2], dB=gr.dB[:2], dC=gr.dC[:2], dh0=gr.dinitial_state[:2],
+                         dA=gr.dA / n, dskip=gr.dD / n, ddbias=gr.ddelta_bias / n))
+    assert not torch.equal(runs[0]["y"], runs[1]["y"])                    # two ways of computing it
+    mags = []
+    for b in range(2):
+        n = int(lens[b])
+        wide = lambda t: np.repeat(t[b, :n].double().numpy()[:, None], D, axis=1)                 # noqa: E731
+        a = dict(x=_np(i["x"][b, :n]), delta=_np(i["delta"][b, :n]), A=_np(i["A"]), B=wide(i["B"]), C=wide(i["C"]), skip=_np(i["D"]),
+                 z=_np(i["z"][b, :n]), dbias=_np(i["delta_bias"]), h0=_np(h0[b]), dy=_np(dy[b, :n]), dend=_np(dend[b]))
+        m = R.scan(**a, mag=True)
+        m["dB"], m["dC"] = m["dB"].sum(1), m["dC"].sum(1)
+        k = 16 * n + 32 + N                          # each of the two is off by as much: twice
+        for name in ("y", "end", "dx", "ddelta", "dz", "dB", "dC", "dh0"):
+            u, v = (_np(r[name][b]) for r in runs)
+            if name not in ("end", "dh0"):
+                u, v = u[:n], v[:n]
+            R.close(u, v, m[name], 2 * k if name in ("y", "end") else 2 * (2 * k + D), what=name)
+        mags.append(m)
+    for name in ("dA", "dskip", "ddbias"):
+        R.close(_np(runs[0][name]), _np(runs[1][name]), mags[0][name] + mags[1][name], 2 * (2 * (16 * T + 32 + N) + T + many), what=name)
+
+
+@pytest.mark.parametrize("N,layout,lens", [(40, "batch", (300, 190)), (64, "rows", (0, 260, 140)), (33, "time", (515,))])
+def test_scan_of_many_states_split_over_time(N, layout, lens):
+    bt = Batch(lens, 20, "f32", layout, seed=N)
+    i, h0 = _scan_inputs(bt, N, 2, True, True)
+    dy, dend, kw = bt.seqs(20), bt.par(bt.B, 20, N), dict(initial_state=h0, **bt.kw)
+    y, end, tape = ssm.selective_scan_train(**i, want_final_state=True, **kw)
+    gr = ssm.selective_scan_backward(**i, dy=dy, tape=tape, dfinal_state=dend, **kw)
+    _check_scan(bt, i, h0, 2, True, dy, dend, y, end, gr)
