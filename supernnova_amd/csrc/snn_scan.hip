@@ -165,13 +165,12 @@ __global__ void __launch_bounds__(256) scan_order_kernel(const snn_seq seq, int*
     if (lane == 0) order[rank] = b;
 }
 
-// h 2^p + v, p cut to what takes any h to 0 or inf.  2^p itself would overflow for p >= 128 (the decay over a chunk of growing
-// states) where its product with a small h does not: the whole part of p goes to the exponent of h.
+// h 2^p + v.  2^p itself would overflow for p >= 128 (the decay over a chunk of growing states) where its product with a small h does
+// not: the whole part of p goes to the exponent of h.  At 1000 and -1000 any h is inf or 0 already; a NaN stays.
 struct Pow2 { float frac; int whole; };
 __device__ __forceinline__ Pow2 pow2_parts(float p)
 {
-    const float q = p < -1000.0f ? -1000.0f : (p > 1000.0f ? 1000.0f : p);                  // a NaN stays
-    const float w = fminf(fmaxf(floorf(p), -1000.0f), 1000.0f);
+    const float q = p > 1000.0f ? 1000.0f : p, w = fmaxf(floorf(q), -1000.0f);
     return Pow2{__builtin_amdgcn_exp2f(q - w), (int)w};
 }
 __device__ __forceinline__ float decayed(float h, const Pow2& e, float v) { return fmaf(e.frac, ldexpf(h, e.whole), v); }
