@@ -488,7 +488,8 @@ int snn_sgd_step_clipped(int64_t n, float *params, const float *grads, float *mo
  * kernels only; values out of range are cut to the tensors (a length to [0, max_T], an offset to [0, n_rows]).
  * Rows that belong to no step -- behind a sequence's end in a padded batch, outside every sequence among ragged rows, past
  * max_T -- are never read, and zero in every output.  A sequence of length 0 hands its initial state on.  Offsets must not
- * decrease (the results of a batch whose offsets do are not defined; nothing outside the tensors is touched).  At most 2^24 - 1 sequences, 2^30 steps, 2^19 channels.
+ * decrease (the results of a batch whose offsets do are not defined; nothing outside the tensors is touched).
+ * At most 2^24 - 1 sequences, 2^30 steps, 2^19 channels.
  */
 typedef struct snn_seq {
     int32_t n_seq, max_T;
@@ -509,8 +510,8 @@ typedef struct snn_view {
  * or none.  Steps before the first come from state_in (n_seq, width - 1, channels; NULL: zeros); state_out receives the
  * last width - 1 inputs of every sequence (state_in included where the sequence is shorter) and must not alias state_in.
  * snn_conv_backward: dy, and dstate_out (gradient of state_out) or NULL -> dx, dweight (channels, width), dbias (or NULL),
- * dstate_in (or NULL).  Sums over sequences and steps are taken in a fixed order, the last stage in fp64.  ws:
- * snn_conv_workspace_bytes(args) bytes, 8-byte aligned.
+ * dstate_in (or NULL).  Sums over sequences and steps are taken in an order that depends on the sizes,
+ * the layout and the alignment alone, the last stage in fp64.  ws: snn_conv_workspace_bytes(args) bytes, 8-byte aligned.
  */
 typedef struct snn_conv_args {
     snn_seq seq;
@@ -562,7 +563,7 @@ int64_t snn_scan_tape_floats(const snn_scan_args *args);
 int64_t snn_scan_workspace_bytes(const snn_scan_args *args, int32_t backward);
 int snn_scan_forward(const snn_scan_args *args, void *stream);
 /* Gradients of a scalar loss from dy = dloss/dy (and dstate_out) and the tape of snn_scan_forward over the same inputs.
- * Deterministic: every sum is taken in an order that depends on the sizes alone. */
+ * Deterministic: every sum is taken in an order that depends on the sizes, the layout and the sequences' lengths alone. */
 int snn_scan_backward(const snn_scan_args *args, void *stream);
 /* One step of n_seq sequences: x, delta, z, y (n_seq, channels), B, C (n_seq, groups, states), row stride stride_n;
  * state_in -> state_out, which may be the same buffer. */

@@ -138,14 +138,14 @@ template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_
     clear_rows<T, V>(p.y, fill_of_chunk(p.seq, r, b, c, p.tc, p.sh < 0 && c == p.nc - 1), yb);
 }
 
-// A thread takes the chunks slot, slot + slots, .. so that the parameter gradients of many sequences add up in registers;
-// part[slot][W + 1][D] is summed by conv_bwd_sum_kernel.
+// A thread takes the chunks slot, slot + slots, .. so that the parameter gradients of many sequences add up in registers (fp32: their
+// rounding grows with the chunks of a slot); part[slot][W + 1][D] is summed by conv_bwd_sum_kernel in fp64.
 template <typename T, int V, int W> __global__ void __launch_bounds__(256) conv_bwd_kernel(const ConvP<T> p)
 {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= (int64_t)p.slots * p.cv) return;
     const int slot = (int)(id / p.cv), d = (int)(id - (int64_t)slot * p.cv) * V;
-    float wt[W][V], bs[V], dws[W][V], dbs[V];     // sums over the chunks; a chunk's own come first, so that long sums stay exact
+    float wt[W][V], bs[V], dws[W][V], dbs[V];     // fp32 sums over a slot's chunks; a chunk's own come first: two short chains
     load_taps<V, W>(p.weight, p.bias, d, wt, bs);
     zero_v(dbs);
 #pragma unroll

@@ -10,7 +10,7 @@
 // multiplication that takes them.
 constexpr int SCAN_SEG = 16;                                              // steps per staged segment, forward
 // Steps between the states kept on the tape = steps per segment of the backward, which holds h and a of a segment in
-// registers: 64 of them.  16 steps of K = 4 would be 128, and spill 230 bytes a lane at two waves a SIMD.
+// registers: 64 of them.  16 steps of K = 4 would be 128, and spill 230 bytes a lane at two waves a SIMD (64: up to 84 bytes).
 __host__ __device__ constexpr int scan_tape_steps(int states) { return states <= 8 ? 16 : 8; }
 template <int K> struct ScanTape { static constexpr int STEPS = K == 2 ? 16 : 8; };
 static inline int scan_lanes(int states) { return states <= 16 ? 4 : states <= 32 ? 8 : 16; }

@@ -7,11 +7,12 @@
 // The vector unit bounds the scan, not the memory; so the state stays in registers, everything per step is done once per
 // quad of lanes and not once per lane, and nothing is computed twice unless there is too little to do at once:
 // where channels x sequences do not fill the chip, the time axis is cut into chunks that run side by side.  Then
-// scan_state_kernel finds every chunk's last state from a zero start (and the sum of its steps: the decay over the
+// scan_fwd_kernel<STATE_ONLY> finds every chunk's last state from a zero start (and the sum of its steps: the decay over the
 // whole chunk is exp(A sum s)), scan_combine_kernel runs over the chunks, and scan_fwd_kernel starts each chunk from its
 // true state: 1.7 times the time of a single pass that filled the chip, over `nc` times the lanes.
-// One prompt of 8191 x 4096 bf16, 16 states: 111 + 7 + 171 us, 22 and 33 vector instructions a lane's step of four states where the
-// formula takes 16 and 20, the vector unit busy 0.96 and 0.89 of the time.  16384 sequences of up to 40 x 64 fp32: 120 us.
+// One prompt of 8191 x 4096 bf16, 16 states: 111 + 8 + 172 us, 22 and 33 vector instructions a lane's step of four states where the
+// formula's (step, channel, state) terms take 16 and 20: the rest is per step (softplus, gate, sums over the states, conversions, loads
+// and stores).  The vector unit is busy 0.96 and 0.89 of the time.  16384 sequences of up to 40 x 64 fp32: 120 us.
 #include <algorithm>
 #include "snn_host.h"
 #include "snn_scan.h"
@@ -287,7 +288,9 @@ int snn_scan_check(const snn_scan_args* a, const char* fn)
 // (512 workgroups): whole calls of 1024 steps x 4096 channels bf16, split / not, 138 / 148 us at 256 workgroups, 185 / 194 at
 // 384, 234 / 195 at 512.  Below that, as many chunks as bring the grid to 2048 workgroups, none shorter than 64 steps; 4096 for
 // sequences of different lengths, whose empty chunks leave the chip half full otherwise.  scan_combine_kernel walks over the chunks
-// one by one.  State pass + combination + scan in us, grids of 1024 / 2048 / 4096 / 8192 workgroups: one prompt of 8191 x 4096
+// one by one.  The count takes every sequence for one of max_T steps, so one long sequence among short ones is not split once they
+// are 512 workgroups together, and then runs on its own ones alone: 8192 rows x 4096 bf16 261 us, with six sequences of 64 522, with
+// seven (512 workgroups) 1302.  State pass + combination + scan in us, grids of 1024 / 2048 / 4096 / 8192 workgroups: one prompt of 8191 x 4096
 // bf16 124 + 5 + 194 / 111 + 7 + 171 / 112 + 12 + 174 / 106 + 19 + 177; seven ragged prompts of up to 1501 x 1536 fp16
 // 52 + 5 + 78 / 43 + 5 + 59 / 37 + 7 + 54 / 35 + 11 + 52.
 ScanGrid snn_scan_grid(const snn_scan_args* a)

@@ -9,12 +9,15 @@
 // the adjoint over it; neither is ever divided by a decay.  Sums over states are two DPP adds a quad, dealt over it; sums over
 // channels (dB, dC: 2K values a lane and step) are folded over the wave by v_permlane32_swap / v_permlane16_swap, each of which
 // halves the number of live values while it adds, then DPP rotations, then LDS over the four waves, then -- layers wider than
-// one workgroup's channels -- fp32 partial rows per channel block, added in order by scan_bc_sum_kernel.  Parameter gradients stay in registers over
-// all chunks a workgroup takes and are summed in fp64, in order, by scan_param_sum_kernel.  No atomics.
+// one workgroup's channels -- fp32 partial rows per channel block, added in order by scan_bc_sum_kernel.  Parameter gradients stay
+// in fp32 registers: sums of at most 256 steps, then one addition for each such block over all chunks a workgroup takes, so that the
+// rounding grows with the number of blocks and not of steps; scan_param_sum_kernel adds the workgroups' in fp64, in order.  No atomics.
 //
 // The vector unit bounds it: 108 instructions a lane's step of four states (27 to recompute, 56 for the adjoint, of which the
-// channel sums take 22 issue slots; the rest per segment), at two waves a SIMD (256 registers; three or four waves spill: 880
-// and 1254 us instead of 297).  4 x 2048 x 2048 bf16 of 16 states: adjoint pass 63, combination 6, this kernel 301, sums 8 + 17 us;
+// channel sums take 22 issue slots; 25 per segment and chunk), at two waves a SIMD.  At their 256 registers it spills a little:
+// gated bf16 of 16 states 12 vector registers into 52 bytes of scratch (8 states 16 into 68, fp32 up to 20 into 84), and 222 scalars
+// (twelve views of 64-bit strides live through the time loop) into lanes of vector registers: 38 of a segment's instructions, 5 a
+// step, bring them back, and some 190 a chunk.  Three or four waves a SIMD spill far more: 880 and 1254 us instead of 297.  4 x 2048 x 2048 bf16 of 16 states: adjoint pass 63, combination 6, this kernel 301, sums 8 + 17 us;
 // 512 x 300 x 256 fp32: 323 us, sums 6 + 22 us.
 #include <algorithm>
 #include "snn_host.h"
@@ -56,7 +59,7 @@ template <int K, int LN> __device__ __forceinline__ void channel_sums(float (&b)
     }
 }
 
-// floats of one slot's parameter gradients: dA (D, 4K), dskip (D), dbias (D), and up to 16 bytes
+// floats of one slot's parameter gradients: dA (D, NP), dskip (D), dbias (D), and up to 16 bytes
 __host__ __device__ __forceinline__ int64_t part_stride(int D, int NP) { return ((int64_t)D * (NP + 2) + 3) / 4 * 4; }
 
 // What chunk c > 0 sends back from a zero adjoint, a_{t0} q_{t0}, into carry[b][c - 1], and the sum of its steps into csum[b][c].
@@ -152,7 +155,7 @@ template <typename T, int K, int LN, bool GATE> __global__ void __launch_bounds_
     const ScanCh ch = scan_channel<K, LN>(cb, p.cbg, p.dg, tid);
     const int j = ch.j, d = ch.d;
     const int left_ch = p.dg - (cb - ch.g * p.cbg) * CH, d0 = ch.g * p.dg + p.dg - left_ch;
-    float A2[K], dAs[K], dsks = 0.0f, dbss = 0.0f;      // sums over blocks of 256 steps; a block's own come first, so that long sums stay exact
+    float A2[K], dAs[K], dsks = 0.0f, dbss = 0.0f;      // sums over blocks of 256 steps; a block's own come first
     load_states<K>(p.A + (int64_t)d * p.N, ch.n, p.N, p.vec, A2);
     decay_rates<K>(A2);
 #pragma unroll

@@ -10,8 +10,8 @@ may be strided (a slice of a wider projection needs no copy):
     (T, B, D)  time_major=True (default), padded, `lengths` int32 (B,) on the device or None
     (B, T, D)  time_major=False, padded, `lengths` likewise
     (R, D)     ragged rows, `offsets` int64 (B + 1,) on the device: sequence b holds rows offsets[b] .. offsets[b + 1];
-               `max_len`: a bound on the lengths known to the host (default: the number of rows; the scan splits the time axis by it,
-               so a loose one costs time)
+               `max_len`: a bound on the lengths known to the host (default: the number of rows; the scan cuts the time axis by it
+               as if all sequences were that long: a loose one, or one long sequence among many short ones, costs time)
 Rows that belong to no step (behind a sequence's end, outside every sequence, past max_len) are never read, and zero in every
 output.  A sequence of length 0 hands its initial state on.  Lengths and offsets stay on the device (no synchronisation);
 values out of range are cut to the tensors.  Offsets must not decrease: the results of a batch whose offsets do are not defined.
@@ -225,7 +225,7 @@ def causal_conv_forward(x, weight, bias=None, *, activation="silu", lengths=None
 def causal_conv_backward(x, weight, bias, dy, *, dfinal_state=None, activation="silu", lengths=None, offsets=None, max_len=None,
                          initial_state=None, time_major=True):
     """Gradients of causal_conv_forward's result from dy = dloss/dy and, if the final state was used, dfinal_state.  Sums over
-    sequences and steps are taken in an order that depends on the sizes alone."""
+    sequences and steps are taken in an order that depends on the sizes, the layout and the alignment alone."""
     if _ad._current_level >= 0:
         E._no_tangents(x, weight, bias, dy, dfinal_state, initial_state)
     bt = _Batch(x, lengths, offsets, max_len, time_major)
@@ -247,7 +247,7 @@ def causal_conv_backward(x, weight, bias, dy, *, dfinal_state=None, activation="
 
 def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_state=None):
     """The convolution's output for one new input x (B, D) of every sequence; `state` (B, W - 1, D) holds the inputs before
-    it and is moved on in place, or left as it is and its successor written to `new_state`."""
+    it and is moved on in place, or left as it is and its successor written to `new_state`.  No gradient."""
     if _ad._current_level >= 0:
         E._no_tangents(x, state, weight, bias, new_state)
     bt = _Step(x)
@@ -331,7 +331,7 @@ def selective_scan_forward(x, delta, A, B, C, D=None, z=None, delta_bias=None, *
 def selective_scan_train(x, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_softplus=True, lengths=None, offsets=None,
                          max_len=None, initial_state=None, want_final_state=False, time_major=True):
     """selective_scan_forward that also returns the tape selective_scan_backward starts from: (y, final state or None, tape).
-    The tape holds a state every 16 / 8 / 4 steps for up to 8 / 16 / 64 states."""
+    The tape holds a state every 16 steps for up to 8 states, every 8 steps for more."""
     return _scan_forward(x, delta, A, B, C, D, z, delta_bias, delta_softplus, lengths, offsets, max_len, initial_state,
                          want_final_state, time_major, True)
 
@@ -339,7 +339,7 @@ def selective_scan_train(x, delta, A, B, C, D=None, z=None, delta_bias=None, *, 
 def selective_scan_backward(x, delta, A, B, C, dy, tape, D=None, z=None, delta_bias=None, *, dfinal_state=None, delta_softplus=True,
                             lengths=None, offsets=None, max_len=None, initial_state=None, time_major=True):
     """Gradients from dy = dloss/dy and, if the final state was used, dfinal_state, with the tape of selective_scan_train over the
-    same inputs.  Every sum is taken in an order that depends on the sizes alone."""
+    same inputs.  Every sum is taken in an order that depends on the sizes, the layout and the sequences' lengths alone."""
     if _ad._current_level >= 0:
         E._no_tangents(x, delta, A, B, C, dy, tape, D, z, delta_bias, dfinal_state, initial_state)
     bt = _Batch(x, lengths, offsets, max_len, time_major)
@@ -364,7 +364,7 @@ def selective_scan_backward(x, delta, A, B, C, dy, tape, D=None, z=None, delta_b
 
 def selective_scan_step(x, state, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_softplus=True, new_state=None):
     """One step of every sequence: x, delta, z (B, D), B, C (B, [G,] N); `state` (B, D, N) float32 is moved on in place, or left as
-    it is and its successor written to `new_state`.  Returns y (B, D)."""
+    it is and its successor written to `new_state`.  Returns y (B, D).  No gradient."""
     if _ad._current_level >= 0:
         E._no_tangents(x, state, delta, A, B, C, D, z, delta_bias, new_state)
     bt = _Step(x)
