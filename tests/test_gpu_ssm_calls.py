@@ -327,3 +327,89 @@ def test_scan_of_many_states_split_over_time(N, layout, lens):
     y, end, tape = ssm.selective_scan_train(**i, want_final_state=True, **kw)
     gr = ssm.selective_scan_backward(**i, dy=dy, tape=tape, dfinal_state=dend, **kw)
     _check_scan(bt, i, h0, 2, True, dy, dend, y, end, gr)
+
+
+def _layer(p, kw):
+    u = ssm.causal_conv(p["x"], p["w"], p["b"], **kw)
+    return ssm.selective_scan(u, p["delta"], p["A"], p["B"], p["C"], p["D"], p["z"], p["dtb"], **kw)
+
+
+def _layer_inputs(seed, R_, D=24, N=6):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=g).cuda()                                           # noqa: E731
+    return dict(x=rnd(R_, D), delta=rnd(R_, D), z=rnd(R_, D), B=rnd(R_, N), C=rnd(R_, N), w=rnd(D, 4) / 2, b=rnd(D), A=-torch.rand(D, N, generator=g).cuda() - 0.1,
+                D=rnd(D), dtb=rnd(D) / 2), rnd(R_, D)
+
+
+def test_differentiable_forms_of_rows():
+    """Rows with offsets and no max_len through autograd: the explicit calls' bits, twice over one graph, on a side stream, and
+    padded to (T, B, D) the same values."""
+    lens = [5, 0, 70, 1, 130]
+    off = torch.tensor(np.cumsum([0] + lens)).cuda()
+    i, dy = _layer_inputs(5, sum(lens))
+    kw = dict(offsets=off)
+    u, _ = ssm.causal_conv_forward(i["x"], i["w"], i["b"], **kw)
+    args = dict(x=u, delta=i["delta"], A=i["A"], B=i["B"], C=i["C"], D=i["D"], z=i["z"], delta_bias=i["dtb"])
+    y, _, tape = ssm.selective_scan_train(**args, **kw)
+    gs = ssm.selective_scan_backward(**args, dy=dy, tape=tape, **kw)
+    gc = ssm.causal_conv_backward(i["x"], i["w"], i["b"], gs.dx, **kw)
+    want = dict(x=gc.dx, w=gc.dweight, b=gc.dbias, delta=gs.ddelta, A=gs.dA, B=gs.dB, C=gs.dC, D=gs.dD, z=gs.dz, dtb=gs.ddelta_bias)
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), side):
+        p = {k: v.clone().requires_grad_() for k, v in i.items()}
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            out = _layer(p, kw)
+        torch.cuda.current_stream().wait_stream(stream)
+        first = torch.autograd.grad(out, list(p.values()), dy, retain_graph=True)
+        again = torch.autograd.grad(out, list(p.values()), dy)
+        torch.cuda.synchronize()
+        assert torch.equal(out, y)
+        for k, a, b in zip(p, first, again):
+            assert torch.equal(a, want[k]) and torch.equal(b, want[k]), k
+    T, B = max(lens), len(lens)
+    at = torch.cat([torch.arange(n) * B + b for b, n in enumerate(lens)]).cuda()
+    per = ("x", "delta", "z", "B", "C")
+    p = {k: v.new_zeros(T * B, v.shape[1]).index_copy(0, at, v).view(T, B, -1) if k in per else v for k, v in i.items()}
+    p = {k: v.clone().requires_grad_() for k, v in p.items()}
+    out = _layer(p, dict(lengths=torch.tensor(lens, dtype=torch.int32).cuda()))
+    grads = torch.autograd.grad(out, list(p.values()), dy.new_zeros(T * B, dy.shape[1]).index_copy(0, at, dy).view(T, B, -1))
+    # the same sums cut elsewhere: (32 T + 64) roundings of magnitudes that a random layer of this size holds below 10 times the values
+    tol = 10 * (32 * T + 64) * R.EPS32
+    for k, v in zip(p, grads):
+        v = v.reshape(T * B, -1)[at] if k in per else v
+        assert float((v - want[k]).abs().max()) <= tol * float(want[k].abs().max()), k
+
+
+def test_two_threads_at_once():
+    """Two threads, each with its own stream and sizes: the bits of one after the other."""
+    import threading
+    cases = []
+    for seed, lens in ((1, [300, 20, 44]), (2, [9] * 600)):
+        i, dy = _layer_inputs(seed, sum(lens))
+        cases.append((i, dy, dict(offsets=torch.tensor(np.cumsum([0] + lens)).cuda(), max_len=max(lens))))
+
+    def run(i, dy, kw):
+        p = {k: v.clone().requires_grad_() for k, v in i.items()}
+        out = _layer(p, kw)
+        grads = list(torch.autograd.grad(out, list(p.values()), dy))
+        norm = E.clip_grads(grads, 0.5)
+        return [out.detach(), norm, *grads]
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    got, streams = [[], []], [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def work(n):
+        with torch.cuda.stream(streams[n]):
+            for _ in range(5):
+                got[n].append(run(*cases[n]))
+        streams[n].synchronize()
+    threads = [threading.Thread(target=work, args=(n,)) for n in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for n in (0, 1):
+        assert len(got[n]) == 5
+        for outs in got[n]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[n]))
